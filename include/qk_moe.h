@@ -271,6 +271,58 @@ QKM_API int qkm_dense_upload(qkm_ctx *c, uint32_t slot, uint32_t type, const voi
                              uint32_t M, uint32_t K);
 QKM_API int qkm_dense_gemm(qkm_ctx *c, uint32_t slot, const float *x, uint32_t n, float *y);
 
+/* ---- products with 8-bit floating-point weights (no counterpart in the reference, which has ggml formats only) ---------
+ * Weights as FP8 checkpoints hold them: E4M3 bytes (1 sign, 4 exponent, 3 mantissa bits; 0x7F and 0xFF are NaN, there is no
+ * infinity), row-major [M][K], with one f32 scale for each block of 128 x 128, [ceil(M/128)][ceil(K/128)]; a stack of experts
+ * lies one after the other, scales too.  Activation rows are E4M3 [n][K] with one f32 scale for each 128 columns,
+ * [n][ceil(K/128)]:
+ *   y[n][m] = sum over column blocks b of  x_scale[n][b] * w_scale[m/128][b] * (sum over the block's columns of xq * wq)
+ * The products of one block are added by the tensor cores, the blocks in f32.  M is any number, K a multiple of 16 (the last block
+ * may be short); E4M3 rows start on 16-byte boundaries.  All pointers are DEVICE pointers, scales any f32.  A NaN code makes the sums that it
+ * meets NaN, whatever it is multiplied with, and nothing else.
+ *
+ * qkm_fp8_quantize makes such rows: the scale of 128 columns is the smallest power of two (2^-126 at least, 1 for zeros) that keeps
+ * their largest finite magnitude at or below 448, so that x / scale is exact and an element is rounded once, to nearest even.
+ * Elements that are not finite become NaN. */
+QKM_API int qkm_fp8_quantize(qkm_ctx *c, const float *x, uint32_t n, uint32_t K, void *q, float *scale);
+QKM_API int qkm_fp8_gemm(qkm_ctx *c, const void *W, const float *w_scale, const void *xq,
+                         const float *x_scale, float *y, uint32_t M, uint32_t K, uint32_t n);
+/* The experts' products, as qkm_moe_gateup_grouped, qkm_moe_down_grouped, qkm_moe_shared_gateup and qkm_moe_shared_down with
+ * the context's n_embd, n_ff, n_expert and n_used.  xq: the tokens' rows [n_tokens][n_embd]; hq: rows [n_tokens][n_used + 1][n_ff], e.g.
+ * qkm_fp8_quantize of h with n = n_tokens * (n_used + 1).  gate/up writes the slots that the list names (the shared form slot n_used),
+ * f32; down multiplies by the record's routing weight (w_shared).  Pairs that name a token or a slot that there is none of are skipped. */
+QKM_API int qkm_moe_gateup_grouped_fp8(qkm_ctx *c, const void *gate_exps, const float *gate_scale,
+                                       const void *up_exps, const float *up_scale, const void *xq,
+                                       const float *x_scale, const uint32_t *offsets,
+                                       const uint32_t *pairs, float *h, uint32_t n_tokens);
+QKM_API int qkm_moe_down_grouped_fp8(qkm_ctx *c, const void *down_exps, const float *down_scale,
+                                     const void *hq, const float *h_scale, const qkm_sel *sel,
+                                     const uint32_t *offsets, const uint32_t *pairs, float *contrib,
+                                     uint32_t n_tokens);
+QKM_API int qkm_moe_shared_gateup_fp8(qkm_ctx *c, const void *gate_shexp, const float *gate_scale,
+                                      const void *up_shexp, const float *up_scale, const void *xq,
+                                      const float *x_scale, float *h, uint32_t n_tokens);
+QKM_API int qkm_moe_shared_down_fp8(qkm_ctx *c, const void *down_shexp, const float *down_scale,
+                                    const void *hq, const float *h_scale, const qkm_sel *sel, float *y2,
+                                    uint32_t n_tokens);
+
+/* ---- the router's load (no counterpart in the reference) --------------------------------------------------------------
+ * Balance loss of a batch, and what it is made of:
+ *   loss = coef * E / (N * n_used) * sum_e counts[e] * probs[e]          (coef where every expert gets the same)
+ * N: tokens whose mask byte is not zero (mask NULL: all of them); counts[e]: how many of their selections (sel[t].ids[0..n_used), as
+ * qkm_moe_select writes them; ids past the table are not counted) name expert e; probs[e]: the mean over these tokens of
+ * softmax(logits[t])[e].  A logit that is not finite counts as -3.4e38, as in the selection.  counts: u32[n_expert + 1], the last one N;
+ * probs f32[n_expert]; loss f32[1].  N = 0: all zero.  The result does not depend on the order in which blocks run.  n_tokens <= 2^24.
+ * (Sums in progress lie in the context: two graphs that captured calls of one context must not replay at the same time.) */
+QKM_API int qkm_moe_balance(qkm_ctx *c, const float *logits, const qkm_sel *sel, const uint8_t *mask,
+                            uint32_t n_tokens, float coef, uint32_t *counts, float *probs, float *loss);
+/* d_logits[t][e] = d loss / d logits[t][e] times *d_loss (device f32; NULL: 1), from the counts of qkm_moe_balance (or their sums over
+ * the ranks of a data-parallel batch); the counts have no gradient.  Zero for tokens that the mask leaves out and for
+ * logits that are not finite.  d_logits may be logits. */
+QKM_API int qkm_moe_balance_grad(qkm_ctx *c, const float *logits, const uint8_t *mask,
+                                 const uint32_t *counts, uint32_t n_tokens, float coef,
+                                 const float *d_loss, float *d_logits);
+
 /* ---- GGUF files (src/gguf.h:54-198; tensor set and checks of loadMoeT, src/main.cpp:1265-1308)
  * Read-only, memory-mapped; a split model is opened by its first shard
  * ("<prefix>-00001-of-000NN.gguf").  Every length in the file is bounds-checked; failures

@@ -95,6 +95,14 @@ SIGNATURES = {
     "qkm_upload_layer_gguf": (_I, [_VP, _U32, _VP, _U32]),
     "qkm_dense_upload": (_I, [_VP, _U32, _U32, _VP, _U32, _U32]),
     "qkm_dense_gemm": (_I, [_VP, _U32, _VP, _U32, _VP]),
+    "qkm_fp8_quantize": (_I, [_VP, _VP, _U32, _U32, _VP, _VP]),
+    "qkm_fp8_gemm": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _U32, _U32, _U32]),
+    "qkm_moe_gateup_grouped_fp8": (_I, [_VP] + [_VP] * 9 + [_U32]),
+    "qkm_moe_down_grouped_fp8": (_I, [_VP] + [_VP] * 8 + [_U32]),
+    "qkm_moe_shared_gateup_fp8": (_I, [_VP] + [_VP] * 7 + [_U32]),
+    "qkm_moe_shared_down_fp8": (_I, [_VP] + [_VP] * 6 + [_U32]),
+    "qkm_moe_balance": (_I, [_VP, _VP, _VP, _VP, _U32, C.c_float, _VP, _VP, _VP]),
+    "qkm_moe_balance_grad": (_I, [_VP, _VP, _VP, _VP, _U32, C.c_float, _VP, _VP]),
     "qkm_argmax": (_I, [_VP, _VP, _U32, _U32, _VP]),
     "qkm_add_rmsnorm": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _U32, _U32, C.c_float]),
     "qkm_add_rms3": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _U32, _U32, C.c_float]),
@@ -333,6 +341,49 @@ class Context:
 
     def dense_gemm(self, slot, x, n, y):
         rc = self._calls.dense_gemm(self.h, slot, x, n, y)
+        if rc:
+            self.check(rc)
+
+    # -- products with E4M3 weights (a scale for each block of 128 x 128)
+    def fp8_quantize(self, x, n, K, q, scale):
+        rc = self._calls.fp8_quantize(self.h, x, n, K, q, scale)
+        if rc:
+            self.check(rc)
+
+    def fp8_gemm(self, W, w_scale, xq, x_scale, y, M, K, n=1):
+        rc = self._calls.fp8_gemm(self.h, W, w_scale, xq, x_scale, y, M, K, n)
+        if rc:
+            self.check(rc)
+
+    def moe_gateup_grouped_fp8(self, gate, gate_scale, up, up_scale, xq, x_scale, offsets, pairs, h, n):
+        rc = self._calls.moe_gateup_grouped_fp8(self.h, gate, gate_scale, up, up_scale, xq, x_scale, offsets, pairs, h, n)
+        if rc:
+            self.check(rc)
+
+    def moe_down_grouped_fp8(self, down, down_scale, hq, h_scale, sel, offsets, pairs, contrib, n):
+        rc = self._calls.moe_down_grouped_fp8(self.h, down, down_scale, hq, h_scale, sel, offsets, pairs, contrib, n)
+        if rc:
+            self.check(rc)
+
+    def moe_shared_gateup_fp8(self, gate, gate_scale, up, up_scale, xq, x_scale, h, n):
+        rc = self._calls.moe_shared_gateup_fp8(self.h, gate, gate_scale, up, up_scale, xq, x_scale, h, n)
+        if rc:
+            self.check(rc)
+
+    def moe_shared_down_fp8(self, down, down_scale, hq, h_scale, sel, y2, n):
+        rc = self._calls.moe_shared_down_fp8(self.h, down, down_scale, hq, h_scale, sel, y2, n)
+        if rc:
+            self.check(rc)
+
+    # -- the router's load
+    def moe_balance(self, logits, sel, mask, n, coef, counts, probs, loss):
+        rc = self._calls.moe_balance(self.h, logits, sel, mask, n, coef, counts, probs, loss)
+        if rc:
+            self.check(rc)
+
+    def moe_balance_grad(self, logits, mask, counts, n, coef, d_loss, d_logits):
+        """Gradient of moe_balance's loss with respect to the logits; d_loss: device scalar or None (1)."""
+        rc = self._calls.moe_balance_grad(self.h, logits, mask, counts, n, coef, d_loss, d_logits)
         if rc:
             self.check(rc)
 

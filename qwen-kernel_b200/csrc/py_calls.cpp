@@ -6,6 +6,10 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <tuple>
+#include <type_traits>
+#include <utility>
+
 #include "../../include/qk_moe.h"
 
 namespace {
@@ -94,6 +98,28 @@ PyObject* layer_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// Any C ABI call: pointers, 32-bit numbers and floats in the order of its parameters.
+bool convert(PyObject* o, uint32_t* out) { return u32(o, out); }
+bool convert(PyObject* o, float* out) { return f32(o, out); }
+template <class T>
+bool convert(PyObject* o, T** out) {
+    void* p = nullptr;
+    if (!pointer(o, &p)) return false;
+    *out = (T*)p;
+    return true;
+}
+template <auto F> struct Plain;
+template <class... A, int (*F)(A...)>
+struct Plain<F> {
+    static PyObject* call(PyObject*, PyObject* const* a, Py_ssize_t n) { return with(a, n, std::index_sequence_for<A...>{}); }
+    template <size_t... I>
+    static PyObject* with(PyObject* const* a, Py_ssize_t n, std::index_sequence<I...>) {
+        std::tuple<std::remove_const_t<A>...> v;
+        if (!count("call", n, sizeof...(A)) || !(convert(a[I], &std::get<I>(v)) && ...)) return nullptr;
+        return run([&] { return F(std::get<I>(v)...); });
+    }
+};
+
 #define FAST(f) ((PyCFunction)(void (*)(void))(f))
 PyMethodDef methods[] = {
     {"gemv", FAST(gemv), METH_FASTCALL, nullptr},
@@ -104,6 +130,14 @@ PyMethodDef methods[] = {
     {"moe_decode_stack_host", FAST(stack_call<qkm_moe_decode_stack_host>), METH_FASTCALL, nullptr},
     {"argmax", FAST(argmax), METH_FASTCALL, nullptr},
     {"moe_layer_step", FAST(layer_step), METH_FASTCALL, nullptr},
+    {"fp8_quantize", FAST(Plain<qkm_fp8_quantize>::call), METH_FASTCALL, nullptr},
+    {"fp8_gemm", FAST(Plain<qkm_fp8_gemm>::call), METH_FASTCALL, nullptr},
+    {"moe_gateup_grouped_fp8", FAST(Plain<qkm_moe_gateup_grouped_fp8>::call), METH_FASTCALL, nullptr},
+    {"moe_down_grouped_fp8", FAST(Plain<qkm_moe_down_grouped_fp8>::call), METH_FASTCALL, nullptr},
+    {"moe_shared_gateup_fp8", FAST(Plain<qkm_moe_shared_gateup_fp8>::call), METH_FASTCALL, nullptr},
+    {"moe_shared_down_fp8", FAST(Plain<qkm_moe_shared_down_fp8>::call), METH_FASTCALL, nullptr},
+    {"moe_balance", FAST(Plain<qkm_moe_balance>::call), METH_FASTCALL, nullptr},
+    {"moe_balance_grad", FAST(Plain<qkm_moe_balance_grad>::call), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "qkm_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -16,6 +16,7 @@
 
 #include "qkm_alloc.h"
 #include "qkm_common.cuh"
+#include "qkm_fp8.cuh"
 #include "qkm_kernels.h"
 #include "qkm_tiles.cuh"
 
@@ -95,6 +96,7 @@ struct qkm_ctx {
     uint32_t* pos_of = nullptr;       // [max_tokens*(n_used+1)]
     uint32_t* group_counts = nullptr; // [resident experts] pairs, then [max_tokens*n_used] a pair's number inside its expert
     void* argmax_scratch = nullptr; uint32_t argmax_rows = 0;
+    void* balance_acc = nullptr;      // sums of qkm_moe_balance between its blocks, zero outside it
     // dense matrices for qkm_dense_gemm (tile-ordered copies) and its scratch, sized on demand
     static constexpr int kDenseSlots = 16;
     struct Dense { uint32_t type = 0, M = 0, K = 0; float w_scale = 1.f; void* tiles = nullptr; } dense[kDenseSlots];
@@ -393,6 +395,11 @@ extern "C" QKM_API qkm_ctx* qkm_open(const qkm_config* cfg, char* err, size_t er
         return nullptr;
     }
     *c->status_host = 0;
+    if ((e = cudaMalloc(&c->balance_acc, balance_scratch_bytes())) != cudaSuccess || (e = cudaMemset(c->balance_acc, 0, balance_scratch_bytes())) != cudaSuccess) {
+        bail("qkm_open: balance sums", cudaGetErrorString(e));
+        qkm_close(c);
+        return nullptr;
+    }
     {
         const Launch L0{nullptr, nullptr};
         if ((e = cudaMalloc((void**)&c->lut_pf, wgemm_table_bytes())) != cudaSuccess ||
@@ -418,7 +425,7 @@ extern "C" QKM_API void qkm_close(qkm_ctx* c) {
         if (l.router_norm2) cudaFree(l.router_norm2);
     }
     for (auto& dm : c->dense) if (dm.tiles) cudaFree(dm.tiles);
-    void* scratch[] = {c->argmax_scratch, c->dense_xb, c->dense_scale, c->sel, c->h, c->route_scratch, c->offsets, c->pairs, c->contrib, c->y2, c->x_stage, c->y_stage,
+    void* scratch[] = {c->balance_acc, c->argmax_scratch, c->dense_xb, c->dense_scale, c->sel, c->h, c->route_scratch, c->offsets, c->pairs, c->contrib, c->y2, c->x_stage, c->y_stage,
                        c->stack_x, c->stack_y, c->xscale, c->n_items, c->status, c->route_counter,
                        c->planes8, c->lut_gu, c->lut_dd, c->lut_pf, c->dec_one.mem, c->dec_many.mem,
                        c->xb, c->xnorm, c->hb, c->hscale, c->contrib_p, c->mma_items[0], c->mma_items[1],
@@ -1103,6 +1110,100 @@ extern "C" QKM_API int qkm_dense_gemm(qkm_ctx* c, uint32_t slot, const float* x,
         c->dense_cap_rows = n;
     }
     QKM_LAUNCH(c, launch_dense_gemm(c->L(), dm.type, dm.tiles, dm.w_scale, dm.M, dm.K, x, n, y, c->dense_xb, c->dense_scale, c->lut_pf, (uint32_t)c->n_sms, c->status));
+    return QKM_OK;
+}
+
+// ---------------------------------------------------------------- products with E4M3 weights
+
+namespace {
+
+// The context's device for the calls below, the caller's again afterwards.
+struct OnDevice {
+    int was = -1;
+    explicit OnDevice(int device) {
+        int now = -1;
+        if (cudaGetDevice(&now) == cudaSuccess && now != device && cudaSetDevice(device) == cudaSuccess) was = now;
+    }
+    ~OnDevice() { if (was >= 0) cudaSetDevice(was); }
+};
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+int fp8_product(qkm_ctx* c, const char* name, int mode, const void* w0, const float* s0, const void* w1, const float* s1, const void* xq, const float* xs, const uint32_t* offsets,
+                const uint32_t* pairs, const qkm_sel* sel, float* out, uint32_t M, uint32_t K, uint32_t n) {
+    if (K == 0 || K % 16) return fail(c, QKM_ERR_ARG, "%s: K=%u must be a multiple of 16", name, K);
+    if (!aligned16(w0) || !aligned16(w1) || !aligned16(xq)) return fail(c, QKM_ERR_ARG, "%s: E4M3 rows must start on 16 bytes", name);
+    if (n >= 1u << 28) return fail(c, QKM_ERR_BOUNDS, "%s: %u rows exceed 2^28", name, n);
+    OnDevice on(c->device);
+    Fp8Args a{};
+    a.w[0] = (const uint8_t*)w0; a.w[1] = (const uint8_t*)w1; a.w_scale[0] = s0; a.w_scale[1] = s1;
+    a.xq = (const uint8_t*)xq; a.x_scale = xs; a.offsets = offsets; a.pairs = pairs; a.sel = sel; a.out = out;
+    a.M = M; a.K = K; a.n = n; a.n_experts = c->ecount; a.n_used = c->cfg.dims.n_used; a.status = c->status;
+    QKM_LAUNCH(c, launch_fp8_product(c->L(), mode, a, (uint32_t)c->n_sms));
+    return QKM_OK;
+}
+
+}  // namespace
+
+extern "C" QKM_API int qkm_fp8_quantize(qkm_ctx* c, const float* x, uint32_t n, uint32_t K, void* q, float* scale) {
+    if (!c || !x || !q || !scale) return QKM_ERR_ARG;
+    if (K == 0 || K % 16) return fail(c, QKM_ERR_ARG, "qkm_fp8_quantize: K=%u must be a multiple of 16", K);
+    if (!aligned16(x) || !aligned16(q)) return fail(c, QKM_ERR_ARG, "qkm_fp8_quantize: x and q must start on 16 bytes");
+    OnDevice on(c->device);
+    QKM_LAUNCH(c, launch_fp8_quantize(c->L(), x, n, K, q, scale));
+    return QKM_OK;
+}
+
+extern "C" QKM_API int qkm_fp8_gemm(qkm_ctx* c, const void* W, const float* w_scale, const void* xq, const float* x_scale, float* y, uint32_t M, uint32_t K, uint32_t n) {
+    if (!c || !W || !w_scale || !xq || !x_scale || !y) return QKM_ERR_ARG;
+    return fp8_product(c, "qkm_fp8_gemm", kFp8Dense, W, w_scale, nullptr, nullptr, xq, x_scale, nullptr, nullptr, nullptr, y, M, K, n);
+}
+
+extern "C" QKM_API int qkm_moe_gateup_grouped_fp8(qkm_ctx* c, const void* gate, const float* gate_scale, const void* up, const float* up_scale, const void* xq,
+                                                  const float* x_scale, const uint32_t* offsets, const uint32_t* pairs, float* h, uint32_t n) {
+    if (!c || !gate || !gate_scale || !up || !up_scale || !xq || !x_scale || !offsets || !pairs || !h) return QKM_ERR_ARG;
+    const qkm_dims& d = c->cfg.dims;
+    return fp8_product(c, "qkm_moe_gateup_grouped_fp8", kFp8GateUp, gate, gate_scale, up, up_scale, xq, x_scale, offsets, pairs, nullptr, h, d.n_ff, d.n_embd, n);
+}
+
+extern "C" QKM_API int qkm_moe_down_grouped_fp8(qkm_ctx* c, const void* down, const float* down_scale, const void* hq, const float* h_scale, const qkm_sel* sel,
+                                                const uint32_t* offsets, const uint32_t* pairs, float* contrib, uint32_t n) {
+    if (!c || !down || !down_scale || !hq || !h_scale || !sel || !offsets || !pairs || !contrib) return QKM_ERR_ARG;
+    const qkm_dims& d = c->cfg.dims;
+    return fp8_product(c, "qkm_moe_down_grouped_fp8", kFp8Down, down, down_scale, nullptr, nullptr, hq, h_scale, offsets, pairs, sel, contrib, d.n_embd, d.n_ff, n);
+}
+
+extern "C" QKM_API int qkm_moe_shared_gateup_fp8(qkm_ctx* c, const void* gate, const float* gate_scale, const void* up, const float* up_scale, const void* xq,
+                                                 const float* x_scale, float* h, uint32_t n) {
+    if (!c || !gate || !gate_scale || !up || !up_scale || !xq || !x_scale || !h) return QKM_ERR_ARG;
+    const qkm_dims& d = c->cfg.dims;
+    return fp8_product(c, "qkm_moe_shared_gateup_fp8", kFp8SharedGateUp, gate, gate_scale, up, up_scale, xq, x_scale, nullptr, nullptr, nullptr, h, d.n_ff, d.n_embd, n);
+}
+
+extern "C" QKM_API int qkm_moe_shared_down_fp8(qkm_ctx* c, const void* down, const float* down_scale, const void* hq, const float* h_scale, const qkm_sel* sel, float* y2,
+                                               uint32_t n) {
+    if (!c || !down || !down_scale || !hq || !h_scale || !sel || !y2) return QKM_ERR_ARG;
+    const qkm_dims& d = c->cfg.dims;
+    return fp8_product(c, "qkm_moe_shared_down_fp8", kFp8SharedDown, down, down_scale, nullptr, nullptr, hq, h_scale, nullptr, nullptr, sel, y2, d.n_embd, d.n_ff, n);
+}
+
+// ---------------------------------------------------------------- the router's balance loss
+
+extern "C" QKM_API int qkm_moe_balance(qkm_ctx* c, const float* logits, const qkm_sel* sel, const uint8_t* mask, uint32_t n, float coef, uint32_t* counts, float* probs,
+                                       float* loss) {
+    if (!c || !logits || !sel || !counts || !probs || !loss) return QKM_ERR_ARG;
+    if (n > 1u << 24) return fail(c, QKM_ERR_BOUNDS, "qkm_moe_balance: %u tokens exceed 2^24", n);
+    OnDevice on(c->device);
+    QKM_LAUNCH(c, launch_balance(c->L(), c->cfg.dims, logits, sel, mask, n, coef, c->balance_acc, counts, probs, loss, (uint32_t)c->n_sms));
+    return QKM_OK;
+}
+
+extern "C" QKM_API int qkm_moe_balance_grad(qkm_ctx* c, const float* logits, const uint8_t* mask, const uint32_t* counts, uint32_t n, float coef, const float* d_loss,
+                                            float* d_logits) {
+    if (!c || !logits || !counts || !d_logits) return QKM_ERR_ARG;
+    if (n > 1u << 24) return fail(c, QKM_ERR_BOUNDS, "qkm_moe_balance_grad: %u tokens exceed 2^24", n);
+    OnDevice on(c->device);
+    QKM_LAUNCH(c, launch_balance_grad(c->L(), c->cfg.dims, logits, mask, counts, n, coef, d_loss, d_logits, (uint32_t)c->n_sms));
     return QKM_OK;
 }
 

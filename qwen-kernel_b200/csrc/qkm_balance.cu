@@ -1,0 +1,213 @@
+// The router's balance loss: counts of the selections, mean softmax probabilities, their product, and its gradient.
+//
+//   loss = coef * E / (N k) * sum_e counts[e] * P[e],   P[e] = 1/N * sum over the counted tokens t of p[t][e],   p = softmax over the E logits
+//   d loss / d logit[t][j] = p[t][j] * (g[j] - sum_e p[t][e] g[e]),   g[e] = d_loss * coef * E / (N^2 k) * counts[e]
+//
+// N: tokens that the mask leaves.  The counts have no gradient.  A logit that is not finite is taken as -3.4e38, as the selection takes it
+// (shaders/moe_select.comp:28-34), and gets none.  A warp holds a row in registers, the same columns in the same lane for every row, so a lane adds up its
+// columns' probabilities - and keeps its columns' g - in registers.
+#include <type_traits>
+
+#include "qkm_common.cuh"
+#include "qkm_kernels.h"
+
+namespace qkm {
+namespace {
+
+constexpr int kBalThreads = 256, kBalWarps = kBalThreads / 32;
+constexpr float kFloor = -3.4e38f;
+// Sums over blocks are added as integers of 2^-38: whatever their order, the result is the same.  n_tokens <= 2^24 keeps them inside 64 bits.
+constexpr double kFix = 274877906944.0;
+
+// what balance_kernel keeps between its blocks; all zero before and after a launch
+struct BalanceAcc {
+    unsigned long long p[512];
+    uint32_t counts[512];
+    uint32_t kept, ticket;
+};
+
+// V values a lane: column of value i
+template <bool VEC> __device__ __forceinline__ uint32_t bal_col(uint32_t lane, int i) { return VEC ? ((i >> 2) * 32 + lane) * 4 + (i & 3) : i * 32 + lane; }
+
+// a row's logits -> exp(logit - largest), 0 past the end; returns 1 / their sum; fine: bit i is set where value i's logit is finite
+template <int V, bool VEC>
+__device__ __forceinline__ float row_exp(const float* __restrict__ row, uint32_t E, uint32_t lane, float (&v)[V], uint32_t& fine) {
+    if (VEC) {
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) {
+            const uint32_t c = bal_col<VEC>(lane, 4 * j);
+            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c < E) f = *reinterpret_cast<const float4*>(row + c);
+            v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = bal_col<VEC>(lane, i) < E ? row[bal_col<VEC>(lane, i)] : 0.f;
+    }
+    float most = -INFINITY;
+    fine = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if (isfinite(v[i])) fine |= 1u << i;
+        else v[i] = kFloor;
+        if (bal_col<VEC>(lane, i) < E) most = fmaxf(most, v[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        v[i] = bal_col<VEC>(lane, i) < E ? expf(v[i] - most) : 0.f;
+        sum += v[i];
+    }
+    return 1.f / warp_sum(sum);
+}
+
+template <int V, bool VEC>
+__global__ void __launch_bounds__(kBalThreads)
+balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel, const uint8_t* __restrict__ mask, uint32_t n_tokens, uint32_t E, uint32_t n_used, float coef,
+               BalanceAcc* acc, uint32_t* __restrict__ counts, float* __restrict__ probs, float* __restrict__ loss) {
+    __shared__ float s_p[kBalWarps][V * 32];
+    __shared__ uint32_t s_cnt[V * 32];
+    __shared__ uint32_t s_kept, s_last;
+    __shared__ double s_sum[kBalWarps];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    for (uint32_t i = tid; i < V * 32; i += kBalThreads) s_cnt[i] = 0;
+    if (tid == 0) s_kept = 0;
+    pdl_trigger();
+    pdl_wait();
+    __syncthreads();
+    float p[V] = {};
+    uint32_t kept = 0;
+    for (uint32_t t = blockIdx.x * kBalWarps + warp; t < n_tokens; t += gridDim.x * kBalWarps) {
+        if (mask && mask[t] == 0) continue;
+        float v[V];
+        uint32_t fine;
+        const float inv = row_exp<V, VEC>(logits + (size_t)t * E, E, lane, v, fine);
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] += v[i] * inv;
+        if (lane < n_used) {
+            const uint32_t id = sel[t].ids[lane];
+            if (id < E) atomicAdd(&s_cnt[id], 1u);
+        }
+        ++kept;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) s_p[warp][bal_col<VEC>(lane, i)] = p[i];
+    if (lane == 0 && kept) atomicAdd(&s_kept, kept);
+    __syncthreads();
+    for (uint32_t e = tid; e < E; e += kBalThreads) {
+        double s = 0;
+        for (int w = 0; w < kBalWarps; ++w) s += (double)s_p[w][e];
+        if (s != 0) atomicAdd(&acc->p[e], (unsigned long long)__double2ll_rn(s * kFix));
+        if (s_cnt[e]) atomicAdd(&acc->counts[e], s_cnt[e]);
+    }
+    if (tid == 0 && s_kept) atomicAdd(&acc->kept, s_kept);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_last = atomicAdd(&acc->ticket, 1u) == gridDim.x - 1 ? 1u : 0u;
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    const uint32_t N = __ldcg(&acc->kept);
+    const double per = N ? 1.0 / N : 0.0;
+    double sum = 0;
+    for (uint32_t e = tid; e < E; e += kBalThreads) {
+        const double P = (double)__ldcg(&acc->p[e]) * (per / kFix);
+        const uint32_t c = __ldcg(&acc->counts[e]);
+        acc->p[e] = 0; acc->counts[e] = 0;
+        counts[e] = c;
+        probs[e] = (float)P;
+        sum += (double)c * P;
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kBalWarps; ++w) sum += s_sum[w];
+        counts[E] = N;
+        *loss = (float)(sum * per * ((double)coef * E / n_used));
+        acc->kept = 0; acc->ticket = 0;
+    }
+}
+
+template <int V, bool VEC>
+__global__ void __launch_bounds__(kBalThreads)
+balance_grad_kernel(const float* logits, const uint8_t* __restrict__ mask, const uint32_t* __restrict__ counts, uint32_t n_tokens, uint32_t E, uint32_t n_used, float coef,
+                    const float* __restrict__ d_loss, float* d_logits) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t N = counts[E];
+    const double unit = N ? (double)coef * E / n_used / N / N * (d_loss ? (double)*d_loss : 1.0) : 0.0;
+    float g[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[i] = bal_col<VEC>(lane, i) < E ? (float)(unit * counts[bal_col<VEC>(lane, i)]) : 0.f;
+    for (uint32_t t = blockIdx.x * kBalWarps + warp; t < n_tokens; t += gridDim.x * kBalWarps) {
+        float v[V];
+        if (mask && mask[t] == 0) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = 0.f;
+        } else {
+            uint32_t fine;
+            const float inv = row_exp<V, VEC>(logits + (size_t)t * E, E, lane, v, fine);
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) { v[i] *= inv; dot += v[i] * g[i]; }
+            dot = warp_sum(dot);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = fine >> i & 1u ? v[i] * (g[i] - dot) : 0.f;
+        }
+        float* out = d_logits + (size_t)t * E;
+        if (VEC) {
+#pragma unroll
+            for (int j = 0; j < V / 4; ++j)
+                if (bal_col<VEC>(lane, 4 * j) < E)
+                    *reinterpret_cast<float4*>(out + bal_col<VEC>(lane, 4 * j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (bal_col<VEC>(lane, i) < E) out[bal_col<VEC>(lane, i)] = v[i];
+        }
+    }
+}
+
+// f<V, VEC>() for rows of E logits: 4, 8 or 16 values a lane; 16-byte loads where every row starts on 16 bytes
+template <class F>
+cudaError_t bal_variant(uint32_t E, bool vec, F f) {
+    if (E <= 128) return vec ? f(std::integral_constant<int, 4>{}, std::true_type{}) : f(std::integral_constant<int, 4>{}, std::false_type{});
+    if (E <= 256) return vec ? f(std::integral_constant<int, 8>{}, std::true_type{}) : f(std::integral_constant<int, 8>{}, std::false_type{});
+    return vec ? f(std::integral_constant<int, 16>{}, std::true_type{}) : f(std::integral_constant<int, 16>{}, std::false_type{});
+}
+uint32_t bal_grid(uint32_t n_tokens, uint32_t n_sms, uint32_t per_sm) {
+    const uint32_t want = (n_tokens + kBalWarps - 1) / kBalWarps;
+    return want < 1 ? 1u : want < n_sms * per_sm ? want : n_sms * per_sm;
+}
+
+}  // namespace
+
+size_t balance_scratch_bytes() { return sizeof(BalanceAcc); }
+
+cudaError_t launch_balance(const Launch& L, const qkm_dims& d, const float* logits, const qkm_sel* sel, const uint8_t* mask, uint32_t n_tokens, float coef, void* scratch,
+                           uint32_t* counts, float* probs, float* loss, uint32_t n_sms) {
+    const cudaError_t e = bal_variant(d.n_expert, d.n_expert % 4 == 0 && ((uintptr_t)logits & 15u) == 0, [&](auto v, auto vec) {
+        return launch_kernel(Launch{L.stream, nullptr, true}, balance_kernel<v.value, vec.value>, dim3(bal_grid(n_tokens, n_sms, 2)), dim3(kBalThreads), 0, logits, sel, mask,
+                             n_tokens, d.n_expert, d.n_used, coef, (BalanceAcc*)scratch, counts, probs, loss);
+    });
+    L.count();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+cudaError_t launch_balance_grad(const Launch& L, const qkm_dims& d, const float* logits, const uint8_t* mask, const uint32_t* counts, uint32_t n_tokens, float coef,
+                                const float* d_loss, float* d_logits, uint32_t n_sms) {
+    if (n_tokens == 0) return cudaSuccess;
+    const bool vec = d.n_expert % 4 == 0 && (((uintptr_t)logits | (uintptr_t)d_logits) & 15u) == 0;
+    const cudaError_t e = bal_variant(d.n_expert, vec, [&](auto v, auto ve) {
+        return launch_kernel(Launch{L.stream, nullptr, true}, balance_grad_kernel<v.value, ve.value>, dim3(bal_grid(n_tokens, n_sms, 4)), dim3(kBalThreads), 0, logits, mask,
+                             counts, n_tokens, d.n_expert, d.n_used, coef, d_loss, d_logits);
+    });
+    L.count();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace qkm

@@ -1,0 +1,244 @@
+// Products with E4M3 weights, a scale for each block of 128 x 128: the rows' quantiser, and the products of few rows.
+#include "qkm_common.cuh"
+#include "qkm_fp8.cuh"
+
+namespace qkm {
+
+// ---- quantiser: f32 rows -> E4M3 with a power of two for each 128 columns -------------------------------------------------------
+// The scale is the smallest power of two that keeps the block's largest finite magnitude at or below 448 = 1.75 * 2^8, E4M3's largest:
+// dividing by it is exact, so an element is rounded once, by at most 2^-4 of itself (2^-10 of the scale below 2^-6 of it).
+// A warp takes a block of 128 columns, a lane four of them.
+namespace {
+
+constexpr int kQuantThreads = 256;
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    uint16_t lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+    return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+__global__ void __launch_bounds__(kQuantThreads)
+fp8_quantize_kernel(const float* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scale, uint64_t n_blocks, uint32_t K, uint32_t KB) {
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint64_t b = (uint64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
+    pdl_trigger();
+    pdl_wait();
+    if (b >= n_blocks) return;
+    const uint64_t row = b / KB;
+    const uint32_t col = (uint32_t)(b - row * KB) * 128u + lane * 4u;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (col < K) v = *reinterpret_cast<const float4*>(x + row * K + col);
+    float* e = &v.x;
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t m = __float_as_uint(e[i]) & 0x7FFFFFFFu;
+        if (m < 0x7F800000u) most = max(most, m);
+        else e[i] = __uint_as_float(0x7FC00000u);          // E4M3 has no infinity: what is not finite becomes NaN
+    }
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    // 1.75 * 2^E <= 448 * 2^(E - 8): the exponent moves up one where the mantissa is above 1.75
+    const uint32_t up = (most + 0x1FFFFFu) >> 23;
+    const uint32_t eb = most == 0 ? 127u : up > 9u ? up - 8u : 1u;
+    const float inv = __uint_as_float((254u - eb) << 23);
+    if (col < K) *reinterpret_cast<uint32_t*>(q + row * K + col) = e4m3x4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    if (lane == 0) scale[b] = __uint_as_float(eb << 23);
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_quantize(const Launch& L, const float* x, uint32_t n, uint32_t K, void* q, float* scale) {
+    if (n == 0) return cudaSuccess;
+    const uint32_t KB = (K + 127) / 128;
+    const uint64_t blocks = (uint64_t)n * KB, grid = (blocks + kQuantThreads / 32 - 1) / (kQuantThreads / 32);
+    if (grid > 0x7FFFFFFFu) return cudaErrorInvalidValue;
+    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_quantize_kernel, dim3((uint32_t)grid), dim3(kQuantThreads), 0, x, (uint8_t*)q, scale, blocks, K, KB);
+    L.count();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+// ---- products of few rows --------------------------------------------------------------------------------------------------------
+// Warp-level MMAs (m16n8k32) on operands that come straight from global memory: a tile of 16 weight rows x 128 columns is four 16-byte loads a lane,
+// and a lane's 16 consecutive bytes serve as its part of two MMAs - the order in which a sum's columns meet is free as long as both operands
+// take the same one.  The eight warps of a block share a tile's column blocks; their sums meet in shared memory, in a fixed order.
+namespace {
+
+constexpr int kRowsThreads = 256, kRowsWarps = kRowsThreads / 32;
+
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 ld16(const uint8_t* p, bool there) { return there ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0); }
+
+template <int MODE> constexpr int rows_mats() { return MODE == kFp8GateUp || MODE == kFp8SharedGateUp ? 2 : 1; }
+
+// 16 weight rows from m0 of expert e times rows [p0, p0 + 8 NT) of its run; NT: groups of eight rows
+template <int MODE, int NT>
+__device__ __forceinline__ void rows_tile(const Fp8Args& a, uint32_t e, uint32_t m0, uint32_t p0, uint32_t p1, float* s_red) {
+    constexpr int MATS = rows_mats<MODE>();
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
+    const uint32_t KB = fp8_blocks(a.K), MB = fp8_blocks(a.M);
+    const uint8_t* xrow[NT];
+    const float* xsc[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        uint64_t o;
+        float w;
+        const uint32_t p = p0 + 8 * j + g;
+        const uint32_t r = p < p1 ? fp8_row<MODE>(a, p, o, w) : kFp8NoRow;
+        xrow[j] = r == kFp8NoRow ? nullptr : a.xq + (uint64_t)r * a.K;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t pc = p0 + 8 * j + 2 * t + c, rc = pc < p1 ? fp8_row<MODE>(a, pc, o, w) : kFp8NoRow;
+            xsc[j][c] = rc == kFp8NoRow ? nullptr : a.x_scale + (uint64_t)rc * KB;
+        }
+    }
+    const uint8_t* wrow[MATS];
+    const float* wsc[MATS];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) {
+        wrow[m] = a.w[m] + ((uint64_t)e * a.M + m0 + g) * a.K;
+        wsc[m] = a.w_scale[m] + ((uint64_t)e * MB + m0 / 128) * KB;
+    }
+    const bool has0 = m0 + g < a.M, has1 = m0 + g + 8 < a.M;
+    float acc[MATS][NT][4] = {};
+    for (uint32_t kb = warp; kb < KB; kb += kRowsWarps) {
+        const uint32_t c0 = kb * 128 + t * 16;
+        const bool in[2] = {c0 < a.K, c0 + 64 < a.K};
+        uint4 wv[MATS][2][2];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                wv[m][c][0] = ld16(wrow[m] + c0 + 64 * c, has0 && in[c]);
+                wv[m][c][1] = ld16(wrow[m] + (uint64_t)8 * a.K + c0 + 64 * c, has1 && in[c]);
+            }
+        float ws[MATS];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) ws[m] = __ldg(wsc[m] + kb);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            uint4 xv[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) xv[c] = ld16(xrow[j] + c0 + 64 * c, xrow[j] != nullptr && in[c]);
+            const float x0 = xsc[j][0] ? xsc[j][0][kb] : 0.f, x1 = xsc[j][1] ? xsc[j][1][kb] : 0.f;
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) {
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    mma_e4m3(d, wv[m][c][0].x, wv[m][c][1].x, wv[m][c][0].y, wv[m][c][1].y, xv[c].x, xv[c].y);
+                    mma_e4m3(d, wv[m][c][0].z, wv[m][c][1].z, wv[m][c][0].w, wv[m][c][1].w, xv[c].z, xv[c].w);
+                }
+                const float s0 = x0 * ws[m], s1 = x1 * ws[m];
+                acc[m][j][0] += d[0] * s0; acc[m][j][1] += d[1] * s1; acc[m][j][2] += d[2] * s0; acc[m][j][3] += d[3] * s1;
+            }
+        }
+    }
+    // s_red[warp][mat][column][16 rows]
+    constexpr uint32_t kCols = 8 * NT, kTile = MATS * kCols * 16;
+    __syncthreads();   // (the tile before has been read)
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                s_red[warp * kTile + (m * kCols + 8 * j + 2 * t + (i & 1)) * 16 + g + 8 * (i >> 1)] = acc[m][j][i];
+    __syncthreads();
+    for (uint32_t i = tid; i < kCols * 16; i += kRowsThreads) {
+        const uint32_t col = i >> 4, m = m0 + (i & 15u), p = p0 + col;
+        if (p >= p1 || m >= a.M) continue;
+        float v[MATS] = {};
+#pragma unroll
+        for (int mat = 0; mat < MATS; ++mat)
+            for (int w = 0; w < kRowsWarps; ++w) v[mat] += s_red[w * kTile + mat * kCols * 16 + i];
+        uint64_t o;
+        float wt;
+        if (fp8_row<MODE>(a, p, o, wt) == kFp8NoRow) continue;
+        a.out[o * a.M + m] = MATS == 2 ? swiglu(v[0], v[MATS - 1]) : MODE == kFp8Dense ? v[0] : wt * v[0];
+    }
+}
+
+// experts that have pairs, in order; returns how many (the same for all threads)
+__device__ __forceinline__ uint32_t live_experts(const Fp8Args& a, uint16_t* s_live) {
+    __shared__ uint32_t s_cnt[kRowsWarps];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    uint32_t total = 0;
+    for (uint32_t e0 = 0; e0 < a.n_experts; e0 += kRowsThreads) {
+        const uint32_t e = e0 + tid;
+        uint32_t p0 = 0, p1 = 0;
+        if (e < a.n_experts) fp8_run(a, e, p0, p1);
+        const uint32_t b = __ballot_sync(0xFFFFFFFFu, p1 > p0);
+        if (lane == 0) s_cnt[warp] = __popc(b);
+        __syncthreads();
+        uint32_t at = total;
+        for (uint32_t w = 0; w < kRowsWarps; ++w) {
+            if (w < warp) at += s_cnt[w];
+            total += s_cnt[w];
+        }
+        if (p1 > p0) s_live[at + __popc(b & ((1u << lane) - 1u))] = (uint16_t)e;
+        __syncthreads();
+    }
+    return total;
+}
+
+template <int MODE, int NT>
+__global__ void __launch_bounds__(kRowsThreads)
+fp8_rows_kernel(const Fp8Args a) {
+    constexpr uint32_t kCols = 8 * NT;
+    __shared__ float s_red[kRowsWarps * rows_mats<MODE>() * kCols * 16];
+    __shared__ uint16_t s_live[512];
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t tiles = (a.M + 15) / 16;
+    constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    const uint64_t units = (uint64_t)tiles * (kGrouped ? live_experts(a, s_live) : 1u);
+    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const uint32_t i = (uint32_t)(u / tiles), m0 = (uint32_t)(u - (uint64_t)i * tiles) * 16u;
+        uint32_t e = 0, p0 = 0, p1 = a.n;
+        if (kGrouped) { e = s_live[i]; fp8_run(a, e, p0, p1); }
+        for (uint32_t p = p0 + blockIdx.y * kCols; p < p1; p += gridDim.y * kCols) rows_tile<MODE, NT>(a, e, m0, p, p1, s_red);
+    }
+}
+
+template <int MODE>
+cudaError_t rows_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
+    const uint64_t tiles = (a.M + 15) / 16;
+    constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    const uint64_t most = kGrouped ? tiles * a.n_experts : tiles;
+    const Launch P{L.stream, nullptr, true};
+    cudaError_t e;
+    auto go = [&](auto kernel, uint32_t cols) {
+        const uint32_t chunks = kGrouped ? 1u : (a.n + cols - 1) / cols;
+        const uint32_t gx = (uint32_t)(kGrouped ? (most < n_sms * 8ull ? most : n_sms * 8ull) : (most < 0x7FFFFFFF ? most : 0x7FFFFFFF));
+        return launch_kernel(P, kernel, dim3(gx, chunks < 65535 ? chunks : 65535), dim3(kRowsThreads), 0, a);
+    };
+    if (kGrouped ? a.n <= 8 : a.n <= 8) e = go(fp8_rows_kernel<MODE, 1>, 8);
+    else e = go(fp8_rows_kernel<MODE, 2>, 16);
+    L.count();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_rows(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) {
+    if (a.n == 0 || a.M == 0) return cudaSuccess;
+    switch (mode) {
+        case kFp8Dense: return rows_launch<kFp8Dense>(L, a, n_sms);
+        case kFp8GateUp: return rows_launch<kFp8GateUp>(L, a, n_sms);
+        case kFp8Down: return rows_launch<kFp8Down>(L, a, n_sms);
+        case kFp8SharedGateUp: return rows_launch<kFp8SharedGateUp>(L, a, n_sms);
+        case kFp8SharedDown: return rows_launch<kFp8SharedDown>(L, a, n_sms);
+    }
+    return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) { return launch_fp8_rows(L, mode, a, n_sms); }
+
+}  // namespace qkm

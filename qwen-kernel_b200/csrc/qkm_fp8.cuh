@@ -1,0 +1,54 @@
+// E4M3 operands with a scale for each block of 128: what the kernels of qkm_fp8.cu and qkm_fp8_gemm.cu share.
+//
+// A product is  y[row][m] = sum over column blocks b of  x_scale[row][b] * w_scale[m / 128][b] * (sum over the block's columns of xq * wq):
+// the tensor cores add the products of one block, exact to their f32 accumulators, and the block's two scales are applied to that sum in f32.
+#pragma once
+
+#include "qkm_kernels.h"
+#include "qkm_stream.cuh"
+
+namespace qkm {
+
+// Where the activation rows of a unit come from and its results go.  A "pair" is (token << 4) | slot; of the shared expert and of a dense
+// product pair p is row p.
+enum Fp8Mode { kFp8Dense = 0, kFp8GateUp = 1, kFp8Down = 2, kFp8SharedGateUp = 3, kFp8SharedDown = 4 };
+constexpr uint32_t kFp8NoRow = 0xFFFFFFFFu;
+
+struct Fp8Args {
+    const uint8_t* w[2];           // E4M3 rows [experts][M][K]; gate and up, or one matrix
+    const float* w_scale[2];       // [experts][ceil(M / 128)][ceil(K / 128)]
+    const uint8_t* xq;             // E4M3 rows of K
+    const float* x_scale;          // [rows][ceil(K / 128)]
+    const uint32_t *offsets, *pairs;
+    const qkm_sel* sel;            // routing weights of the down products
+    float* out;
+    uint32_t M, K, n;              // n: rows (dense), tokens otherwise
+    uint32_t n_experts, n_used;
+    uint32_t* status;
+};
+
+__device__ __forceinline__ uint32_t fp8_blocks(uint32_t v) { return (v + 127u) / 128u; }
+
+// pair (or row) number p of expert e's run -> row of xq; kFp8NoRow where a list names a token or slot that there is none of
+template <int MODE>
+__device__ __forceinline__ uint32_t fp8_row(const Fp8Args& a, uint32_t p, uint64_t& out_row, float& weight) {
+    weight = 1.f;
+    if (MODE == kFp8Dense) { out_row = p; return p; }
+    if (MODE == kFp8SharedGateUp) { out_row = (uint64_t)p * (a.n_used + 1) + a.n_used; return p; }
+    if (MODE == kFp8SharedDown) { out_row = p; weight = a.sel[p].w_shared; return p * (a.n_used + 1) + a.n_used; }
+    const uint32_t pr = a.pairs[p], t = pr >> 4, s = pr & 15u;
+    if (t >= a.n || s >= a.n_used) { out_row = 0; return kFp8NoRow; }
+    if (MODE == kFp8GateUp) { out_row = (uint64_t)t * (a.n_used + 1) + s; return t; }
+    out_row = (uint64_t)t * a.n_used + s;
+    weight = a.sel[t].w[s];
+    return t * (a.n_used + 1) + s;
+}
+// expert e's run of the list of pairs, whatever the offsets hold inside the list
+__device__ __forceinline__ void fp8_run(const Fp8Args& a, uint32_t e, uint32_t& p0, uint32_t& p1) {
+    const uint32_t most = a.n * a.n_used;
+    p0 = min(a.offsets[e], most);
+    p1 = min(a.offsets[e + 1], most);
+    if (p1 < p0) p1 = p0;
+}
+
+}  // namespace qkm

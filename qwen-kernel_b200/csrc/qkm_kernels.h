@@ -338,6 +338,19 @@ cudaError_t launch_add_rms(const Launch& L, int mode, const float* a, const floa
 size_t argmax_scratch_bytes(uint32_t n_rows);
 cudaError_t launch_argmax(const Launch& L, const float* logits, uint32_t n_rows, uint32_t n, void* scratch, uint32_t scratch_rows, uint32_t* tok);
 
+// ---- products with E4M3 weights (qkm_fp8.cu, qkm_fp8_gemm.cu; Fp8Args in qkm_fp8.cuh) ------------------------
+struct Fp8Args;
+cudaError_t launch_fp8_quantize(const Launch& L, const float* x, uint32_t n, uint32_t K, void* q, float* scale);
+cudaError_t launch_fp8_rows(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms);      // few rows
+cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms);   // any number
+
+// ---- the router's balance loss and its gradient (qkm_balance.cu); scratch: balance_scratch_bytes(), zero before the first call
+size_t balance_scratch_bytes();
+cudaError_t launch_balance(const Launch& L, const qkm_dims& d, const float* logits, const qkm_sel* sel, const uint8_t* mask, uint32_t n_tokens, float coef, void* scratch,
+                           uint32_t* counts, float* probs, float* loss, uint32_t n_sms);
+cudaError_t launch_balance_grad(const Launch& L, const qkm_dims& d, const float* logits, const uint8_t* mask, const uint32_t* counts, uint32_t n_tokens, float coef,
+                                const float* d_loss, float* d_logits, uint32_t n_sms);
+
 // ---- expert-parallel exchange helpers (qkm_ep.cu) --------------------------------------------
 // counts[0..n_ranks) rows per destination rank and counts[n_ranks] their sum; send_tok the
 // tokens in send order; send_pos[t][r] the row of token t among the rows sent (to rank r).
