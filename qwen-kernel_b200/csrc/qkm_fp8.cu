@@ -239,6 +239,5 @@ cudaError_t launch_fp8_rows(const Launch& L, int mode, const Fp8Args& a, uint32_
     return cudaErrorInvalidValue;
 }
 
-cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) { return launch_fp8_rows(L, mode, a, n_sms); }
 
 }  // namespace qkm

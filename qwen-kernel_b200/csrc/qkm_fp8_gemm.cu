@@ -1,0 +1,267 @@
+// Products of many rows with E4M3 weights and block scales on the 5th-generation tensor cores (tcgen05, kind::f8f6f4).
+//
+// A tile of y is 128 rows (256 for a pair of blocks) x BN weight rows.  The sum over one block of 128 columns is four MMAs (K = 32 each) into a set of
+// tensor-memory columns of its own; eight warps read the set back, multiply it by the block's two scales and add it to the tile's f32 sums in registers,
+// while the MMAs of the next block run into another set.  Activation rows are the lanes (M), weight rows the columns (N): a thread holds one
+// row and a run of columns inside one block of 128 weight rows, so the scale is one number a thread and the scaling one FMA an element.
+#include <cuda.h>
+
+#include "qkm_common.cuh"
+#include "qkm_fp8.cuh"
+#include "qkm_umma.cuh"
+#include "qkm_wait.h"
+
+namespace qkm {
+namespace {
+
+namespace tg {
+constexpr int kThreads = 384;                    // 4 warps that load and issue, 8 that scale and add
+constexpr int kAux = 4, kAdders = 8;
+constexpr int kRegAux = 40, kRegAdd = 232;       // registers a thread after the split
+static_assert(kAux * 32 * kRegAux + kAdders * 32 * kRegAdd <= kThreads * 168, "the shares must not exceed the launch's registers");
+template <int CG, int BN> struct Tile {
+    static constexpr uint32_t kRowsW = BN / CG;                       // weight rows that a block loads
+    static constexpr uint32_t kStage = 128 * 128 + kRowsW * 128;
+    static constexpr uint32_t kStages = kStage > 32768 ? 4 : 6;
+    static constexpr uint32_t kSets = 512 / BN;                       // tensor-memory column sets
+    static constexpr uint32_t kPut = kStages * kStage;                // 4 KB a warp: the way of the results to coalesced stores
+    static constexpr uint32_t kSmem = kPut + kAdders * 4096 + 1024;   // (+ what aligning the start may take)
+};
+}  // namespace tg
+
+__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, uint32_t x0, uint32_t r0, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x0), "r"(r0), "r"(bar) : "memory");
+}
+// instruction descriptor: E4M3 x E4M3 -> f32, both operands K-major
+__device__ __forceinline__ uint32_t instr_desc_e4m3(uint32_t m, uint32_t n) { return 1u << 4 | (n >> 3) << 17 | (m >> 4) << 24; }
+__device__ __forceinline__ void mma_e4m3_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+    const uint32_t acc = accumulate ? 1u : 0u;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+          "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]),
+          "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr));
+}
+// the registers of a load that has been waited for (keeps their uses behind the wait)
+__device__ __forceinline__ void tmem_ld_done(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]),
+                   "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]),
+                   "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 ::"memory");
+}
+
+struct WideArgs {
+    const float *w_scale, *x_scale;
+    float* y;
+    uint32_t M, n, KB, MB;
+    uint32_t x_tiles, n_tiles;     // tiles along the rows of x; all of them
+    uint32_t vec;                  // 16-byte stores
+    uint32_t* status;
+};
+
+template <int CG, int BN>
+__global__ void __launch_bounds__(tg::kThreads, 1)
+fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map) {
+    using T = tg::Tile<CG, BN>;
+    extern __shared__ uint8_t smem_dyn[];
+    __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets];
+    __shared__ uint32_t s_tmem;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
+    const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * T::kStages, bar_set = bar_empty + 8 * T::kStages, bar_free = bar_set + 8 * T::kSets;
+    if (tid == 0) {
+        for (uint32_t i = 0; i < T::kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < T::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, tg::kAdders); }
+        mbar_fence_init();
+    }
+    if (warp == 2) { umma::tmem_alloc(smem_addr(&s_tmem), 512); umma::tmem_relinquish(); }
+    umma::fence_before_sync();
+    pdl_trigger();
+    pdl_wait();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = s_tmem;
+    Waits waits;
+    auto wait_bar = [&](uint32_t b, uint32_t parity) { waits.wait([&] { return mbar_wait_timed(b, parity); }); };
+
+    if (warp >= (uint32_t)tg::kAux) {
+        // ---- scale and add: TMEM lanes 32 q ..; columns h * BN / 2 ..
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(tg::kRegAdd));
+        constexpr int kCols = BN / 2, kChunks = kCols / 32;
+        const uint32_t q = warp & 3u, h = (warp - tg::kAux) >> 2;
+        const uint32_t put = base + T::kPut + (warp - tg::kAux) * 4096u;
+        uint32_t blk = 0;                                                // column blocks so far: set blk % kSets
+        for (uint32_t u = blockIdx.x; u < a.n_tiles; u += gridDim.x) {
+            const uint32_t xt = u % a.x_tiles, wt = u / a.x_tiles;
+            const uint32_t r0 = xt * 128u + 32 * q, m0 = wt * BN + h * kCols;
+            const float* xs = a.x_scale + (size_t)min(r0 + lane, a.n - 1) * a.KB;
+            const float* ws = a.w_scale + (size_t)min(m0 / 128u, a.MB - 1) * a.KB;
+            float acc[kCols];
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+            float s0 = xs[0] * ws[0], s1 = a.KB > 1 ? xs[1] * ws[1] : 0.f;
+            for (uint32_t kb = 0; kb < a.KB; ++kb, ++blk) {
+                const uint32_t set = blk % T::kSets;
+                const float x2 = kb + 2 < a.KB ? xs[kb + 2] : 0.f, w2 = kb + 2 < a.KB ? ws[kb + 2] : 0.f;
+                wait_bar(bar_set + 8 * set, (blk / T::kSets) & 1u);
+                umma::fence_after_sync();
+                const uint32_t t = tmem + ((32 * q) << 16) + set * BN + h * kCols;
+                float v[2][32];
+                tmem_ld32(t, v[0]);
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    tmem_ld_done(v[c & 1]);
+                    if (c + 1 < kChunks) tmem_ld32(t + 32 * (c + 1), v[(c + 1) & 1]);
+                    else {
+                        umma::fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar_free + 8 * set);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(v[c & 1][i], s0, acc[32 * c + i]);
+                }
+                s0 = s1;
+                s1 = x2 * w2;
+            }
+            if (__any_sync(0xFFFFFFFFu, waits.out)) break;
+            // 32 rows x 32 columns at a time through shared memory: lanes along the columns for the stores
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(put + lane * 128u + ((j ^ (lane & 7u)) << 4)), "f"(acc[32 * c + 4 * j]), "f"(acc[32 * c + 4 * j + 1]),
+                                 "f"(acc[32 * c + 4 * j + 2]), "f"(acc[32 * c + 4 * j + 3]) : "memory");
+                __syncwarp();
+                const uint32_t j = lane & 7u, m = m0 + 32 * c + 4 * j;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t r = 4 * i + (lane >> 3), row = r0 + r;
+                    const uint4 o = lds128(put + r * 128u + ((j ^ (r & 7u)) << 4));
+                    if (row >= a.n) continue;
+                    float* y = a.y + (size_t)row * a.M + m;
+                    if (a.vec) {
+                        if (m < a.M) *reinterpret_cast<uint4*>(y) = o;
+                    } else {
+                        const uint32_t e[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (m + k < a.M) y[k] = __uint_as_float(e[k]);
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(tg::kRegAux));
+        if (warp == 0) {
+            // ---- loads
+            uint32_t it = 0;
+            for (uint32_t u = blockIdx.x; u < a.n_tiles; u += gridDim.x) {
+                const uint32_t xt = u % a.x_tiles, wt = u / a.x_tiles;
+                for (uint32_t kb = 0; kb < a.KB; ++kb, ++it) {
+                    const uint32_t s = it % T::kStages, dst = base + s * T::kStage;
+                    if (it >= T::kStages) wait_bar(bar_empty + 8 * s, (it / T::kStages - 1) & 1u);
+                    if (__any_sync(0xFFFFFFFFu, waits.out)) break;   // a barrier that still counts bytes takes no second arrival
+                    if (lane == 0) {
+                        mbar_expect_tx(bar_full + 8 * s, T::kStage);
+                        tma_tile(dst, &x_map, kb * 128u, xt * 128u, bar_full + 8 * s);
+                        tma_tile(dst + 16384u, &w_map, kb * 128u, wt * BN, bar_full + 8 * s);
+                    }
+                    __syncwarp();
+                }
+            }
+        } else if (warp == 1) {
+            // ---- MMAs
+            const bool leader = umma::elect_one();
+            const uint32_t idesc = instr_desc_e4m3(128, BN);
+            uint32_t it = 0;
+            for (uint32_t u = blockIdx.x; u < a.n_tiles; u += gridDim.x)
+                for (uint32_t kb = 0; kb < a.KB; ++kb, ++it) {
+                    const uint32_t s = it % T::kStages, set = it % T::kSets;
+                    if (it >= T::kSets) wait_bar(bar_free + 8 * set, (it / T::kSets - 1) & 1u);
+                    wait_bar(bar_full + 8 * s, (it / T::kStages) & 1u);
+                    umma::fence_after_sync();
+                    const uint64_t da = umma::smem_desc(base + s * T::kStage), db = umma::smem_desc(base + s * T::kStage + 16384u);
+                    if (leader) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma_e4m3_ss(tmem + set * BN, da + 2 * j, db + 2 * j, idesc, j != 0);
+                        umma::commit(bar_empty + 8 * s);
+                        umma::commit(bar_set + 8 * set);
+                    }
+                    __syncwarp();
+                }
+        }
+    }
+    umma::fence_before_sync();
+    const int any_timed_out = __syncthreads_or(waits.out ? 1 : 0);
+    if (any_timed_out) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies and MMAs still under way end long before this does
+    if (warp == 2) umma::tmem_dealloc(tmem, 512);
+    if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
+}
+
+// tensor map over E4M3 rows [rows][K]: boxes of `box` rows x 128 columns, 128-byte swizzle, zeros outside
+bool fp8_map(CUtensorMap* map, const void* p, uint64_t rows, uint32_t K, uint32_t box) {
+    typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const EncodeFn encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres) == cudaSuccess ? (EncodeFn)fn : (EncodeFn) nullptr;
+    }();
+    if (!encode) return false;
+    const cuuint64_t dim[2] = {K, rows}, stride[1] = {K};
+    const cuuint32_t boxes[2] = {128, box}, estride[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dim, stride, boxes, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The register split needs what the launch bounds promise: less would leave the warps that ask for more waiting for good.
+template <auto Kernel>
+cudaError_t check_registers() {
+    static const int regs = [] {
+        cudaFuncAttributes f{};
+        return cudaFuncGetAttributes(&f, Kernel) == cudaSuccess ? f.numRegs : 0;
+    }();
+    return regs >= 168 ? cudaSuccess : cudaErrorInvalidKernelImage;
+}
+
+template <int CG, int BN>
+cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
+    using T = tg::Tile<CG, BN>;
+    if (const cudaError_t e = allow_dynamic_smem<fp8_wide_kernel<CG, BN>>((int)T::kSmem)) return e;
+    if (const cudaError_t e = check_registers<fp8_wide_kernel<CG, BN>>()) return e;
+    CUtensorMap xm, wm;
+    if (!fp8_map(&xm, a.xq, a.n, a.K, 128) || !fp8_map(&wm, a.w[0], a.M, a.K, T::kRowsW)) return cudaErrorInvalidValue;
+    WideArgs w{};
+    w.w_scale = a.w_scale[0]; w.x_scale = a.x_scale; w.y = a.out; w.M = a.M; w.n = a.n; w.KB = (a.K + 127) / 128; w.MB = (a.M + 127) / 128;
+    w.x_tiles = (a.n + 127) / 128;
+    const uint64_t tiles = (uint64_t)w.x_tiles * ((a.M + BN - 1) / BN);
+    if (tiles > 0x7FFFFFFFu) return cudaErrorInvalidValue;
+    w.n_tiles = (uint32_t)tiles;
+    w.vec = a.M % 4 == 0 && ((uintptr_t)a.out & 15u) == 0;
+    w.status = a.status;
+    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_wide_kernel<CG, BN>, dim3(tiles < n_sms ? (uint32_t)tiles : n_sms), dim3(tg::kThreads), T::kSmem, w, xm, wm);
+    L.count();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) {
+    if (mode == kFp8Dense && a.n > 64 && a.K >= 128 && a.M >= 16) return wide_launch<1, 256>(L, a, n_sms);
+    return launch_fp8_rows(L, mode, a, n_sms);
+}
+
+}  // namespace qkm
