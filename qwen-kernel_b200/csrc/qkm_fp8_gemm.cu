@@ -29,21 +29,73 @@ template <int CG, int BN> struct Tile {
 };
 }  // namespace tg
 
+// a box of rows into this block's shared memory; of a pair (CG 2) the barrier may be the other block's
+template <int CG>
 __device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, uint32_t x0, uint32_t r0, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(x0), "r"(r0), "r"(bar) : "memory");
+    if constexpr (CG == 2)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(x0), "r"(r0), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(x0), "r"(r0), "r"(bar) : "memory");
+}
+// ---- pairs of blocks (cta_group::2): one MMA over both blocks' tiles, issued by the first; both hold half of each operand
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the same shared-memory address in the cluster's first block
+__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+template <int CG> __device__ __forceinline__ void tmem_take(uint32_t smem_dst) {
+    if constexpr (CG == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_dst) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        umma::tmem_alloc(smem_dst, 512);
+        umma::tmem_relinquish();
+    }
+}
+template <int CG> __device__ __forceinline__ void tmem_give_back(uint32_t taddr) {
+    if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+    else umma::tmem_dealloc(taddr, 512);
+}
+// the MMAs issued so far arrive on the barrier at this address of every block of the pair
+template <int CG> __device__ __forceinline__ void commit_all(uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    else
+        umma::commit(bar);
 }
 // instruction descriptor: E4M3 x E4M3 -> f32, both operands K-major
 __device__ __forceinline__ uint32_t instr_desc_e4m3(uint32_t m, uint32_t n) { return 1u << 4 | (n >> 3) << 17 | (m >> 4) << 24; }
+template <int CG>
 __device__ __forceinline__ void mma_e4m3_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
     const uint32_t acc = accumulate ? 1u : 0u;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
-        : "memory");
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+            "}\n" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "setp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+            "}\n" ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+            : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     asm volatile(
@@ -80,17 +132,20 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
     __shared__ uint32_t s_tmem;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0u, unit0 = blockIdx.x / CG, units = gridDim.x / CG;
     const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * T::kStages, bar_set = bar_empty + 8 * T::kStages, bar_free = bar_set + 8 * T::kSets;
     if (tid == 0) {
         for (uint32_t i = 0; i < T::kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
-        for (uint32_t i = 0; i < T::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, tg::kAdders); }
+        for (uint32_t i = 0; i < T::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, CG * tg::kAdders); }
         mbar_fence_init();
     }
-    if (warp == 2) { umma::tmem_alloc(smem_addr(&s_tmem), 512); umma::tmem_relinquish(); }
+    if (warp == 2) tmem_take<CG>(smem_addr(&s_tmem));
     umma::fence_before_sync();
     pdl_trigger();
     pdl_wait();
-    __syncthreads();
+    __syncwarp();
+    if (CG == 2) cluster_sync();
+    else __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = s_tmem;
     Waits waits;
@@ -103,9 +158,9 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
         const uint32_t q = warp & 3u, h = (warp - tg::kAux) >> 2;
         const uint32_t put = base + T::kPut + (warp - tg::kAux) * 4096u;
         uint32_t blk = 0;                                                // column blocks so far: set blk % kSets
-        for (uint32_t u = blockIdx.x; u < a.n_tiles; u += gridDim.x) {
+        for (uint32_t u = unit0; u < a.n_tiles; u += units) {
             const uint32_t xt = u % a.x_tiles, wt = u / a.x_tiles;
-            const uint32_t r0 = xt * 128u + 32 * q, m0 = wt * BN + h * kCols;
+            const uint32_t r0 = (xt * CG + rank) * 128u + 32 * q, m0 = wt * BN + h * kCols;
             const float* xs = a.x_scale + (size_t)min(r0 + lane, a.n - 1) * a.KB;
             const float* ws = a.w_scale + (size_t)min(m0 / 128u, a.MB - 1) * a.KB;
             float acc[kCols];
@@ -127,7 +182,7 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
                     else {
                         umma::fence_before_sync();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(bar_free + 8 * set);
+                        if (lane == 0) { if (CG == 2) mbar_arrive_cluster(in_first(bar_free + 8 * set)); else mbar_arrive(bar_free + 8 * set); }
                     }
 #pragma unroll
                     for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(v[c & 1][i], s0, acc[32 * c + i]);
@@ -168,26 +223,31 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
         if (warp == 0) {
             // ---- loads
             uint32_t it = 0;
-            for (uint32_t u = blockIdx.x; u < a.n_tiles; u += gridDim.x) {
+            for (uint32_t u = unit0; u < a.n_tiles; u += units) {
                 const uint32_t xt = u % a.x_tiles, wt = u / a.x_tiles;
                 for (uint32_t kb = 0; kb < a.KB; ++kb, ++it) {
                     const uint32_t s = it % T::kStages, dst = base + s * T::kStage;
                     if (it >= T::kStages) wait_bar(bar_empty + 8 * s, (it / T::kStages - 1) & 1u);
                     if (__any_sync(0xFFFFFFFFu, waits.out)) break;   // a barrier that still counts bytes takes no second arrival
                     if (lane == 0) {
-                        mbar_expect_tx(bar_full + 8 * s, T::kStage);
-                        tma_tile(dst, &x_map, kb * 128u, xt * 128u, bar_full + 8 * s);
-                        tma_tile(dst + 16384u, &w_map, kb * 128u, wt * BN, bar_full + 8 * s);
+                        // (the first block's barrier counts the bytes of both; the other's may arrive ahead of their announcement, which
+                        // the phase still waits for)
+                        const uint32_t full = CG == 2 ? in_first(bar_full + 8 * s) : bar_full + 8 * s;
+                        if (rank == 0) mbar_expect_tx(bar_full + 8 * s, CG * T::kStage);
+                        tma_tile<CG>(dst, &x_map, kb * 128u, (xt * CG + rank) * 128u, full);
+                        tma_tile<CG>(dst + 16384u, &w_map, kb * 128u, wt * BN + rank * T::kRowsW, full);
                     }
                     __syncwarp();
                 }
             }
-        } else if (warp == 1) {
+            // the MMAs have read everything, and their arrivals here are in
+            for (uint32_t i = it > T::kStages ? it - T::kStages : 0; i < it; ++i) wait_bar(bar_empty + 8 * (i % T::kStages), (i / T::kStages) & 1u);
+        } else if (warp == 1 && rank == 0) {
             // ---- MMAs
             const bool leader = umma::elect_one();
-            const uint32_t idesc = instr_desc_e4m3(128, BN);
+            const uint32_t idesc = instr_desc_e4m3(128 * CG, BN);
             uint32_t it = 0;
-            for (uint32_t u = blockIdx.x; u < a.n_tiles; u += gridDim.x)
+            for (uint32_t u = unit0; u < a.n_tiles; u += units)
                 for (uint32_t kb = 0; kb < a.KB; ++kb, ++it) {
                     const uint32_t s = it % T::kStages, set = it % T::kSets;
                     if (it >= T::kSets) wait_bar(bar_free + 8 * set, (it / T::kSets - 1) & 1u);
@@ -196,9 +256,9 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
                     const uint64_t da = umma::smem_desc(base + s * T::kStage), db = umma::smem_desc(base + s * T::kStage + 16384u);
                     if (leader) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mma_e4m3_ss(tmem + set * BN, da + 2 * j, db + 2 * j, idesc, j != 0);
-                        umma::commit(bar_empty + 8 * s);
-                        umma::commit(bar_set + 8 * set);
+                        for (int j = 0; j < 4; ++j) mma_e4m3_ss<CG>(tmem + set * BN, da + 2 * j, db + 2 * j, idesc, j != 0);
+                        commit_all<CG>(bar_empty + 8 * s);
+                        commit_all<CG>(bar_set + 8 * set);
                     }
                     __syncwarp();
                 }
@@ -207,7 +267,8 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
     umma::fence_before_sync();
     const int any_timed_out = __syncthreads_or(waits.out ? 1 : 0);
     if (any_timed_out) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies and MMAs still under way end long before this does
-    if (warp == 2) umma::tmem_dealloc(tmem, 512);
+    if (CG == 2) cluster_sync();   // nothing of this block is read, written or signalled by the other one any more
+    if (warp == 2) tmem_give_back<CG>(tmem);
     if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
 }
 
@@ -246,13 +307,22 @@ cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     if (!fp8_map(&xm, a.xq, a.n, a.K, 128) || !fp8_map(&wm, a.w[0], a.M, a.K, T::kRowsW)) return cudaErrorInvalidValue;
     WideArgs w{};
     w.w_scale = a.w_scale[0]; w.x_scale = a.x_scale; w.y = a.out; w.M = a.M; w.n = a.n; w.KB = (a.K + 127) / 128; w.MB = (a.M + 127) / 128;
-    w.x_tiles = (a.n + 127) / 128;
+    w.x_tiles = (a.n + 128 * CG - 1) / (128 * CG);
     const uint64_t tiles = (uint64_t)w.x_tiles * ((a.M + BN - 1) / BN);
     if (tiles > 0x7FFFFFFFu) return cudaErrorInvalidValue;
     w.n_tiles = (uint32_t)tiles;
     w.vec = a.M % 4 == 0 && ((uintptr_t)a.out & 15u) == 0;
     w.status = a.status;
-    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_wide_kernel<CG, BN>, dim3(tiles < n_sms ? (uint32_t)tiles : n_sms), dim3(tg::kThreads), T::kSmem, w, xm, wm);
+    const uint32_t grid = CG * (uint32_t)(tiles < n_sms / CG ? tiles : n_sms / CG);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(tg::kThreads); cfg.dynamicSmemBytes = T::kSmem; cfg.stream = L.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CG; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = CG == 2 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_wide_kernel<CG, BN>, w, xm, wm);
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -260,7 +330,7 @@ cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
 }  // namespace
 
 cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) {
-    if (mode == kFp8Dense && a.n > 64 && a.K >= 128 && a.M >= 16) return wide_launch<1, 256>(L, a, n_sms);
+    if (mode == kFp8Dense && a.n > 64 && a.K >= 128 && a.M >= 16) return a.n > 256 ? wide_launch<2, 256>(L, a, n_sms) : wide_launch<1, 256>(L, a, n_sms);
     return launch_fp8_rows(L, mode, a, n_sms);
 }
 
