@@ -18,12 +18,13 @@ namespace tg {
 constexpr int kThreads = 384;                    // 4 warps that load and issue, 8 that scale and add
 constexpr int kAux = 4, kAdders = 8;
 constexpr int kRegAux = 40, kRegAdd = 232;       // registers a thread after the split
-static_assert(kAux * 32 * kRegAux + kAdders * 32 * kRegAdd <= kThreads * 168, "the shares must not exceed the launch's registers");
-template <int CG, int BN> struct Tile {
-    static constexpr uint32_t kRowsW = BN / CG;                       // weight rows that a block loads
+constexpr int kRegLaunch = 168;
+static_assert(kAux * 32 * kRegAux + kAdders * 32 * kRegAdd <= kThreads * kRegLaunch, "the shares must not exceed the launch's registers");
+constexpr uint32_t kBN = 256;                    // weight rows of a tile; CG blocks share a tile of CG * 128 rows
+template <int CG> struct Tile {
+    static constexpr uint32_t kRowsW = kBN / CG;                      // weight rows that a block loads
     static constexpr uint32_t kStage = 128 * 128 + kRowsW * 128;
-    static constexpr uint32_t kStages = kStage > 32768 ? 4 : 6;
-    static constexpr uint32_t kSets = 512 / BN;                       // tensor-memory column sets
+    static constexpr uint32_t kStages = CG == 2 ? 6 : 4;
     static constexpr uint32_t kPut = kStages * kStage;                // 4 KB a warp: the way of the results to coalesced stores
     static constexpr uint32_t kSmem = kPut + kAdders * 4096 + 1024;   // (+ what aligning the start may take)
 };
@@ -54,7 +55,7 @@ __device__ __forceinline__ uint32_t in_first(uint32_t addr) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 template <int CG> __device__ __forceinline__ void tmem_take(uint32_t smem_dst) {
     if constexpr (CG == 2) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_dst) : "memory");
@@ -114,6 +115,34 @@ __device__ __forceinline__ void tmem_ld_done(float (&v)[32]) {
                  ::"memory");
 }
 
+// whether the phase is through, without waiting for it
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// acc += v * s, two elements an instruction
+__device__ __forceinline__ void add_scaled(float (&acc)[64], int at, const float (&v)[32], float s) {
+    uint64_t s2;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
+#pragma unroll
+    for (int i = 0; i < 32; i += 2)
+        asm("{\n"
+            ".reg .b64 v, c;\n"
+            "mov.b64 v, {%2, %3};\n"
+            "mov.b64 c, {%0, %1};\n"
+            "fma.rn.f32x2 c, v, %4, c;\n"
+            "mov.b64 {%0, %1}, c;\n"
+            "}\n"
+            : "+f"(acc[at + i]), "+f"(acc[at + i + 1]) : "f"(v[i]), "f"(v[i + 1]), "l"(s2));
+}
+
 struct WideArgs {
     const float *w_scale, *x_scale;
     float* y;
@@ -123,20 +152,20 @@ struct WideArgs {
     uint32_t* status;
 };
 
-template <int CG, int BN>
+template <int CG>
 __global__ void __launch_bounds__(tg::kThreads, 1)
 fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map) {
-    using T = tg::Tile<CG, BN>;
+    using T = tg::Tile<CG>;
     extern __shared__ uint8_t smem_dyn[];
-    __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets];
+    __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 4];
     __shared__ uint32_t s_tmem;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-    const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0u, unit0 = blockIdx.x / CG, units = gridDim.x / CG;
-    const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * T::kStages, bar_set = bar_empty + 8 * T::kStages, bar_free = bar_set + 8 * T::kSets;
+    const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
+    const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * T::kStages, bar_set = bar_empty + 8 * T::kStages, bar_free = bar_set + 16;
     if (tid == 0) {
         for (uint32_t i = 0; i < T::kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
-        for (uint32_t i = 0; i < T::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, CG * tg::kAdders); }
+        for (uint32_t i = 0; i < 2; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, CG * tg::kAdders); }
         mbar_fence_init();
     }
     if (warp == 2) tmem_take<CG>(smem_addr(&s_tmem));
@@ -149,56 +178,67 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
     umma::fence_after_sync();
     const uint32_t tmem = s_tmem;
     Waits waits;
-    auto wait_bar = [&](uint32_t b, uint32_t parity) { waits.wait([&] { return mbar_wait_timed(b, parity); }); };
+    // A few polls that end at once when the phase does, then such that let the thread sleep (which take 60 cycles more to wake up).
+    auto wait_bar = [&](uint32_t b, uint32_t parity) {
+        waits.wait([&] {
+#pragma unroll 1
+            for (int i = 0; i < 64; ++i)
+                if (mbar_try_wait(b, parity)) return true;
+            return mbar_wait_timed(b, parity);
+        });
+    };
 
     if (warp >= (uint32_t)tg::kAux) {
-        // ---- scale and add: TMEM lanes 32 q ..; columns h * BN / 2 ..
+        // ---- scale and add: TMEM lanes 32 q .., columns 128 h .. of a set, weight rows of one block of 128
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(tg::kRegAdd));
-        constexpr int kCols = BN / 2, kChunks = kCols / 32;
         const uint32_t q = warp & 3u, h = (warp - tg::kAux) >> 2;
         const uint32_t put = base + T::kPut + (warp - tg::kAux) * 4096u;
-        uint32_t blk = 0;                                                // column blocks so far: set blk % kSets
+        const uint32_t t0 = tmem + ((32 * q) << 16) + h * 128u, free0 = CG == 2 ? in_first(bar_free) : bar_free;
+        uint32_t blk = 0;                                                // column blocks so far: set blk % 2
+        bool ready = false;                                              // the next set's barrier is through
         for (uint32_t u = unit0; u < a.n_tiles; u += units) {
             const uint32_t xt = u % a.x_tiles, wt = u / a.x_tiles;
-            const uint32_t r0 = (xt * CG + rank) * 128u + 32 * q, m0 = wt * BN + h * kCols;
+            const uint32_t r0 = (xt * CG + rank) * 128u + 32 * q, m0 = wt * tg::kBN + h * 128u;
             const float* xs = a.x_scale + (size_t)min(r0 + lane, a.n - 1) * a.KB;
             const float* ws = a.w_scale + (size_t)min(m0 / 128u, a.MB - 1) * a.KB;
-            float acc[kCols];
+            float acc[2][64];
 #pragma unroll
-            for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
-            float s0 = xs[0] * ws[0], s1 = a.KB > 1 ? xs[1] * ws[1] : 0.f;
+            for (int i = 0; i < 128; ++i) acc[i >> 6][i & 63] = 0.f;
+            float x0 = xs[0], w0 = ws[0];                                // (the next block's scales are on their way while this one's are used)
             for (uint32_t kb = 0; kb < a.KB; ++kb, ++blk) {
-                const uint32_t set = blk % T::kSets;
-                const float x2 = kb + 2 < a.KB ? xs[kb + 2] : 0.f, w2 = kb + 2 < a.KB ? ws[kb + 2] : 0.f;
-                wait_bar(bar_set + 8 * set, (blk / T::kSets) & 1u);
+                const uint32_t set = blk & 1u, t = t0 + set * 256u;
+                const float xc = x0, wc = w0;
+                if (kb + 1 < a.KB) { x0 = xs[kb + 1]; w0 = ws[kb + 1]; }
+                if (!ready) wait_bar(bar_set + 8 * set, (blk >> 1) & 1u);
                 umma::fence_after_sync();
-                const uint32_t t = tmem + ((32 * q) << 16) + set * BN + h * kCols;
+                const float s = xc * wc;
                 float v[2][32];
                 tmem_ld32(t, v[0]);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c) {
-                    tmem_ld_done(v[c & 1]);
-                    if (c + 1 < kChunks) tmem_ld32(t + 32 * (c + 1), v[(c + 1) & 1]);
-                    else {
-                        umma::fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) { if (CG == 2) mbar_arrive_cluster(in_first(bar_free + 8 * set)); else mbar_arrive(bar_free + 8 * set); }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) acc[32 * c + i] = fmaf(v[c & 1][i], s0, acc[32 * c + i]);
-                }
-                s0 = s1;
-                s1 = x2 * w2;
+                tmem_ld32(t + 32, v[1]);
+                tmem_ld_done(v[0]);
+                tmem_ld_done(v[1]);
+                add_scaled(acc[0], 0, v[0], s);
+                add_scaled(acc[0], 32, v[1], s);
+                tmem_ld32(t + 64, v[0]);
+                tmem_ld32(t + 96, v[1]);
+                tmem_ld_done(v[0]);
+                tmem_ld_done(v[1]);
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) { if (CG == 2) mbar_arrive_cluster(free0 + 8 * set); else mbar_arrive(free0 + 8 * set); }
+                ready = mbar_test(bar_set + 8 * (set ^ 1u), ((blk + 1) >> 1) & 1u);   // its answer comes while the additions run
+                add_scaled(acc[1], 0, v[0], s);
+                add_scaled(acc[1], 32, v[1], s);
             }
             if (__any_sync(0xFFFFFFFFu, waits.out)) break;
             // 32 rows x 32 columns at a time through shared memory: lanes along the columns for the stores
 #pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
+            for (int c = 0; c < 4; ++c) {
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(put + lane * 128u + ((j ^ (lane & 7u)) << 4)), "f"(acc[32 * c + 4 * j]), "f"(acc[32 * c + 4 * j + 1]),
-                                 "f"(acc[32 * c + 4 * j + 2]), "f"(acc[32 * c + 4 * j + 3]) : "memory");
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(put + lane * 128u + ((j ^ (lane & 7u)) << 4)), "f"(acc[c >> 1][32 * (c & 1) + 4 * j]),
+                                 "f"(acc[c >> 1][32 * (c & 1) + 4 * j + 1]), "f"(acc[c >> 1][32 * (c & 1) + 4 * j + 2]), "f"(acc[c >> 1][32 * (c & 1) + 4 * j + 3]) : "memory");
                 __syncwarp();
                 const uint32_t j = lane & 7u, m = m0 + 32 * c + 4 * j;
 #pragma unroll
@@ -235,7 +275,7 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
                         const uint32_t full = CG == 2 ? in_first(bar_full + 8 * s) : bar_full + 8 * s;
                         if (rank == 0) mbar_expect_tx(bar_full + 8 * s, CG * T::kStage);
                         tma_tile<CG>(dst, &x_map, kb * 128u, (xt * CG + rank) * 128u, full);
-                        tma_tile<CG>(dst + 16384u, &w_map, kb * 128u, wt * BN + rank * T::kRowsW, full);
+                        tma_tile<CG>(dst + 16384u, &w_map, kb * 128u, wt * tg::kBN + rank * T::kRowsW, full);
                     }
                     __syncwarp();
                 }
@@ -243,25 +283,30 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
             // the MMAs have read everything, and their arrivals here are in
             for (uint32_t i = it > T::kStages ? it - T::kStages : 0; i < it; ++i) wait_bar(bar_empty + 8 * (i % T::kStages), (i / T::kStages) & 1u);
         } else if (warp == 1 && rank == 0) {
-            // ---- MMAs
+            // ---- MMAs.  The way from a set's return to the next MMA into it is part of the loop that bounds the kernel: as few
+            // instructions as may be, counters that are added to instead of remainders.
             const bool leader = umma::elect_one();
-            const uint32_t idesc = instr_desc_e4m3(128 * CG, BN);
-            uint32_t it = 0;
-            for (uint32_t u = unit0; u < a.n_tiles; u += units)
-                for (uint32_t kb = 0; kb < a.KB; ++kb, ++it) {
-                    const uint32_t s = it % T::kStages, set = it % T::kSets;
-                    if (it >= T::kSets) wait_bar(bar_free + 8 * set, (it / T::kSets - 1) & 1u);
-                    wait_bar(bar_full + 8 * s, (it / T::kStages) & 1u);
-                    umma::fence_after_sync();
-                    const uint64_t da = umma::smem_desc(base + s * T::kStage), db = umma::smem_desc(base + s * T::kStage + 16384u);
-                    if (leader) {
+            const uint32_t idesc = instr_desc_e4m3(128 * CG, tg::kBN);
+            const uint32_t steps = unit0 < a.n_tiles ? ((a.n_tiles - unit0 + units - 1) / units) * a.KB : 0u;
+            const uint64_t da0 = umma::smem_desc(base);
+            uint32_t s = 0, full_parity = 0, set = 0, free_parity = 1;   // (the first pass over the sets waits for the phase before the first)
+            uint64_t da = da0;
+            for (uint32_t i = 0; i < steps; ++i) {
+                wait_bar(bar_full + 8 * s, full_parity);
+                wait_bar(bar_free + 8 * set, free_parity);
+                umma::fence_after_sync();
+                if (leader) {   // (after a wait that ran out the MMAs run on: their operands are in bounds, and the tile is never stored)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) mma_e4m3_ss<CG>(tmem + set * BN, da + 2 * j, db + 2 * j, idesc, j != 0);
-                        commit_all<CG>(bar_empty + 8 * s);
-                        commit_all<CG>(bar_set + 8 * set);
-                    }
-                    __syncwarp();
+                    for (int j = 0; j < 4; ++j) mma_e4m3_ss<CG>(tmem + set * 256u, da + 2 * j, da + 1024 + 2 * j, idesc, j != 0);
+                    commit_all<CG>(bar_set + 8 * set);
+                    commit_all<CG>(bar_empty + 8 * s);
                 }
+                __syncwarp();
+                da += T::kStage / 16;
+                if (++s == T::kStages) { s = 0; da = da0; full_parity ^= 1u; }
+                set ^= 1u;
+                free_parity ^= set ^ 1u;
+            }
         }
     }
     umma::fence_before_sync();
@@ -295,20 +340,20 @@ cudaError_t check_registers() {
         cudaFuncAttributes f{};
         return cudaFuncGetAttributes(&f, Kernel) == cudaSuccess ? f.numRegs : 0;
     }();
-    return regs >= 168 ? cudaSuccess : cudaErrorInvalidKernelImage;
+    return regs >= tg::kRegLaunch ? cudaSuccess : cudaErrorInvalidKernelImage;
 }
 
-template <int CG, int BN>
+template <int CG>
 cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
-    using T = tg::Tile<CG, BN>;
-    if (const cudaError_t e = allow_dynamic_smem<fp8_wide_kernel<CG, BN>>((int)T::kSmem)) return e;
-    if (const cudaError_t e = check_registers<fp8_wide_kernel<CG, BN>>()) return e;
+    using T = tg::Tile<CG>;
+    if (const cudaError_t e = allow_dynamic_smem<fp8_wide_kernel<CG>>((int)T::kSmem)) return e;
+    if (const cudaError_t e = check_registers<fp8_wide_kernel<CG>>()) return e;
     CUtensorMap xm, wm;
     if (!fp8_map(&xm, a.xq, a.n, a.K, 128) || !fp8_map(&wm, a.w[0], a.M, a.K, T::kRowsW)) return cudaErrorInvalidValue;
     WideArgs w{};
     w.w_scale = a.w_scale[0]; w.x_scale = a.x_scale; w.y = a.out; w.M = a.M; w.n = a.n; w.KB = (a.K + 127) / 128; w.MB = (a.M + 127) / 128;
     w.x_tiles = (a.n + 128 * CG - 1) / (128 * CG);
-    const uint64_t tiles = (uint64_t)w.x_tiles * ((a.M + BN - 1) / BN);
+    const uint64_t tiles = (uint64_t)w.x_tiles * ((a.M + tg::kBN - 1) / tg::kBN);
     if (tiles > 0x7FFFFFFFu) return cudaErrorInvalidValue;
     w.n_tiles = (uint32_t)tiles;
     w.vec = a.M % 4 == 0 && ((uintptr_t)a.out & 15u) == 0;
@@ -322,7 +367,7 @@ cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = CG; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = CG == 2 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_wide_kernel<CG, BN>, w, xm, wm);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_wide_kernel<CG>, w, xm, wm);
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -330,7 +375,7 @@ cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
 }  // namespace
 
 cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) {
-    if (mode == kFp8Dense && a.n > 64 && a.K >= 128 && a.M >= 16) return a.n > 256 ? wide_launch<2, 256>(L, a, n_sms) : wide_launch<1, 256>(L, a, n_sms);
+    if (mode == kFp8Dense && a.n > 64 && a.K >= 128 && a.M >= 16) return a.n > 256 ? wide_launch<2>(L, a, n_sms) : wide_launch<1>(L, a, n_sms);
     return launch_fp8_rows(L, mode, a, n_sms);
 }
 
