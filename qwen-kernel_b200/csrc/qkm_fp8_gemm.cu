@@ -317,6 +317,322 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
     if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
 }
 
+// ---- products grouped by expert (and dense ones of a middling number of rows) --------------------------------------------------
+// Weight rows are the lanes here (M = 128) and a run of at most NT pairs the columns, as many as there are: the weights are what has to be read.  A unit is
+// the gate and the up rows of one 128-row tile, or two tiles of one matrix, times a run; blocks take consecutive units, so that the runs of an expert
+// with more than NT pairs read a tile from the L2.  Weight tiles come by TMA, the rows of the pairs with 16-byte copies, each row's scale of a
+// column block beside them; the eight warps that scale and add take the row scales from shared memory.
+namespace gg {
+constexpr int kThreads = 512;                    // warps: 0 weights, 1 MMAs, 2 tensor memory, 4 - 7 rows, 8 - 15 scale and add
+constexpr int kRegAux = 40, kRegRows = 56, kRegAdd = 208;
+constexpr int kRegLaunch = 128;
+static_assert(128 * (kRegAux + kRegRows) + 256 * kRegAdd <= kThreads * kRegLaunch, "the shares must not exceed the launch's registers");
+constexpr uint32_t kMaxExperts = 512, kScales = 8;
+template <int NT> struct Tile {
+    static constexpr uint32_t kStage = 2 * 16384 + NT * 128;
+    static constexpr uint32_t kStages = NT > 64 ? 4 : 6;
+    static constexpr uint32_t kSets = NT > 64 ? 2 : 4;                 // of 2 NT columns; fewer than the scale slots less the stages
+    static constexpr uint32_t kSetCols = 512 / kSets;
+    static constexpr uint32_t kScale0 = kStages * kStage;              // [kScales][NT] f32
+    static constexpr uint32_t kSmem = kScale0 + kScales * NT * 4 + 1024;
+    static constexpr int kChunk = NT / 4 < 32 ? NT / 4 : 32;           // columns of a load
+    static constexpr int kChunks = NT / 2 / kChunk;                    // loads a warp and matrix
+};
+}  // namespace gg
+
+struct GroupUnit { uint32_t e, m0, p0, n; };     // expert, first weight row, first pair, pairs
+
+__device__ __forceinline__ void tmem_ld8f(uint32_t taddr, float (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_load(uint32_t t, float (&v)[32]) { tmem_ld32(t, v); }
+__device__ __forceinline__ void tmem_load(uint32_t t, float (&v)[8]) { tmem_ld8f(t, v); }
+// waits for the loads, whose registers are used behind it
+template <int N> __device__ __forceinline__ void tmem_done(float (&a)[N], float (&b)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(a[i]), "+f"(b[i]));
+}
+// acc[0..1] += v[0..1] * (x[0..1] * w)
+__device__ __forceinline__ void add2(float& a0, float& a1, float v0, float v1, float x0, float x1, uint64_t w2) {
+    asm("{\n"
+        ".reg .b64 v, c, x;\n"
+        "mov.b64 v, {%2, %3};\n"
+        "mov.b64 c, {%0, %1};\n"
+        "mov.b64 x, {%4, %5};\n"
+        "mul.rn.f32x2 x, x, %6;\n"
+        "fma.rn.f32x2 c, v, x, c;\n"
+        "mov.b64 {%0, %1}, c;\n"
+        "}\n"
+        : "+f"(a0), "+f"(a1) : "f"(v0), "f"(v1), "f"(x0), "f"(x1), "l"(w2));
+}
+__device__ __forceinline__ uint64_t twice(float w) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(w));
+    return r;
+}
+
+template <int MODE, int NT>
+__global__ void __launch_bounds__(gg::kThreads, 1)
+fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1) {
+    using T = gg::Tile<NT>;
+    constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    static_assert(T::kStages + T::kSets <= gg::kScales + 2, "a scale slot comes back before its next use is due");
+    extern __shared__ uint8_t smem_dyn[];
+    __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets + 2 * gg::kScales];
+    __shared__ uint32_t s_tmem, s_scan[16][2], s_n_live, s_n_units;
+    __shared__ uint32_t s_unit[kGrouped ? gg::kMaxExperts + 1 : 2], s_p0[kGrouped ? gg::kMaxExperts : 1], s_p1[kGrouped ? gg::kMaxExperts : 1];
+    __shared__ uint16_t s_live[kGrouped ? gg::kMaxExperts : 1];
+    __shared__ uint64_t s_out[2][NT];                // where a column's results go, ~0: nowhere
+    __shared__ float s_wt[2][NT];
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
+    const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * T::kStages, bar_set = bar_empty + 8 * T::kStages, bar_free = bar_set + 8 * T::kSets;
+    const uint32_t bar_sfull = bar_free + 8 * T::kSets, bar_sfree = bar_sfull + 8 * gg::kScales;
+    if (tid == 0) {
+        for (uint32_t i = 0; i < T::kStages; ++i) { mbar_init(bar_full + 8 * i, 1 + 4); mbar_init(bar_empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < T::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, 8); }
+        for (uint32_t i = 0; i < gg::kScales; ++i) { mbar_init(bar_sfull + 8 * i, 4); mbar_init(bar_sfree + 8 * i, 8); }
+        mbar_fence_init();
+    }
+    if (warp == 2) { umma::tmem_alloc(smem_addr(&s_tmem), 512); umma::tmem_relinquish(); }
+    umma::fence_before_sync();
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t KB = fp8_blocks(a.K), MB = fp8_blocks(a.M), row_units = kGateUp ? (a.M + 127) / 128 : (a.M + 255) / 256;
+    // the list of units: experts that have pairs, their first unit and their run
+    {
+        uint32_t p0 = 0, p1 = 0;
+        if (kGrouped) { if (tid < a.n_experts) fp8_run(a, tid, p0, p1); }
+        else if (tid == 0) p1 = a.n;
+        const uint32_t live = p1 > p0 ? 1u : 0u, mine = (p1 - p0 + NT - 1) / NT * row_units;
+        uint32_t c = live, v = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t c1 = __shfl_up_sync(0xFFFFFFFFu, c, o), v1 = __shfl_up_sync(0xFFFFFFFFu, v, o);
+            if (lane >= (uint32_t)o) { c += c1; v += v1; }
+        }
+        if (lane == 31) { s_scan[warp][0] = c; s_scan[warp][1] = v; }
+        __syncthreads();
+        for (uint32_t w = 0; w < warp; ++w) { c += s_scan[w][0]; v += s_scan[w][1]; }
+        if (live) {
+            const uint32_t i = c - 1;
+            s_live[i] = (uint16_t)tid; s_p0[i] = p0; s_p1[i] = p1; s_unit[i] = v - mine; s_unit[i + 1] = v;   // (the next one writes the same there)
+        }
+        if (tid == gg::kThreads - 1) { s_n_live = c; s_n_units = v; }
+    }
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = s_tmem, n_units = s_n_units;
+    const uint32_t u_first = (uint32_t)((uint64_t)n_units * blockIdx.x / gridDim.x), u_end = (uint32_t)((uint64_t)n_units * (blockIdx.x + 1) / gridDim.x);
+    uint32_t live_i = 0;
+    if (kGrouped && u_first < u_end)   // the expert of the first unit, by halves
+        for (uint32_t step = gg::kMaxExperts / 2; step; step >>= 1)
+            if (live_i + step < s_n_live && s_unit[live_i + step] <= u_first) live_i += step;
+    auto unit_of = [&](uint32_t u, uint32_t& i) -> GroupUnit {
+        while (u >= s_unit[i + 1]) ++i;
+        const uint32_t run = s_p1[i] - s_p0[i], parts = (run + NT - 1) / NT, at = u - s_unit[i], ru = at / parts, part = at - ru * parts;
+        GroupUnit g;
+        g.e = kGrouped ? s_live[i] : 0u;
+        g.m0 = ru * (kGateUp ? 128u : 256u);
+        g.p0 = s_p0[i] + part * NT;
+        g.n = min((uint32_t)NT, run - part * NT);
+        return g;
+    };
+    Waits waits;
+    auto wait_bar = [&](uint32_t b, uint32_t parity) {
+        waits.wait([&] {
+#pragma unroll 1
+            for (int i = 0; i < 64; ++i)
+                if (mbar_try_wait(b, parity)) return true;
+            return mbar_wait_timed(b, parity);
+        });
+    };
+
+    if (warp >= 8) {
+        // ---- scale and add
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(gg::kRegAdd));
+        const uint32_t q = warp & 3u, h = (warp - 8) >> 2, c = tid - 256;
+        uint32_t blk = 0, set = 0, set_parity = 0, parity = 0;
+        for (uint32_t u = u_first; u < u_end; ++u, parity ^= 1u) {
+            const GroupUnit g = unit_of(u, live_i);
+            if (c < g.n) {
+                uint64_t row;
+                float wt;
+                const uint32_t r = fp8_row<MODE>(a, g.p0 + c, row, wt);
+                s_out[parity][c] = r == kFp8NoRow ? ~0ull : row * a.M;
+                s_wt[parity][c] = wt;
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            const float* ws0 = a.w_scale[0] + ((uint64_t)g.e * MB + g.m0 / 128u) * KB;
+            const float* ws1 = kGateUp ? a.w_scale[1] + ((uint64_t)g.e * MB + g.m0 / 128u) * KB : ws0 + (g.m0 / 128u + 1 < MB ? KB : 0u);
+            float acc[2][T::kChunks][T::kChunk];
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int j = 0; j < T::kChunks; ++j)
+#pragma unroll
+                    for (int i = 0; i < T::kChunk; ++i) acc[m][j][i] = 0.f;
+            float w0 = ws0[0], w1 = ws1[0];
+            for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
+                const uint32_t slot = blk % gg::kScales, sc = base + T::kScale0 + slot * NT * 4, t = tmem + ((32 * q) << 16) + set * T::kSetCols;
+                const float wc0 = w0, wc1 = w1;
+                if (kb + 1 < KB) { w0 = ws0[kb + 1]; w1 = ws1[kb + 1]; }
+                wait_bar(lane == 1 ? bar_sfull + 8 * slot : bar_set + 8 * set, lane == 1 ? (blk / gg::kScales) & 1u : set_parity);   // two barriers in one poll
+                __syncwarp();
+                umma::fence_after_sync();
+                const uint64_t wa = twice(wc0), wb = twice(wc1);
+#pragma unroll
+                for (int j = 0; j < T::kChunks; ++j) {
+                    const uint32_t col = (2 * j + h) * T::kChunk;
+                    if (col >= g.n) continue;
+                    float v0[T::kChunk], v1[T::kChunk];
+                    tmem_load(t + col, v0);
+                    tmem_load(t + NT + col, v1);
+                    tmem_done(v0, v1);
+#pragma unroll
+                    for (int i = 0; i < T::kChunk; i += 4) {
+                        const uint4 x = lds128(sc + 4 * (col + i));
+                        const float x0 = __uint_as_float(x.x), x1 = __uint_as_float(x.y), x2 = __uint_as_float(x.z), x3 = __uint_as_float(x.w);
+                        add2(acc[0][j][i], acc[0][j][i + 1], v0[i], v0[i + 1], x0, x1, wa);
+                        add2(acc[0][j][i + 2], acc[0][j][i + 3], v0[i + 2], v0[i + 3], x2, x3, wa);
+                        add2(acc[1][j][i], acc[1][j][i + 1], v1[i], v1[i + 1], x0, x1, wb);
+                        add2(acc[1][j][i + 2], acc[1][j][i + 3], v1[i + 2], v1[i + 3], x2, x3, wb);
+                    }
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(bar_free + 8 * set); mbar_arrive(bar_sfree + 8 * slot); }
+                if (++set == T::kSets) { set = 0; set_parity ^= 1u; }
+            }
+            if (__any_sync(0xFFFFFFFFu, waits.out)) continue;   // (on through the list: the other warps meet this one at the barrier above)
+            const uint32_t m = g.m0 + 32 * q + lane;
+#pragma unroll
+            for (int j = 0; j < T::kChunks; ++j)
+#pragma unroll
+                for (int i = 0; i < T::kChunk; ++i) {
+                    const uint32_t col = (2 * j + h) * T::kChunk + i;
+                    if (col >= g.n) continue;
+                    const uint64_t at = s_out[parity][col];
+                    if (at == ~0ull) continue;
+                    if (kGateUp) {
+                        if (m < a.M) a.out[at + m] = swiglu(acc[0][j][i], acc[1][j][i]);
+                    } else {
+                        const float wt = MODE == kFp8Dense ? 1.f : s_wt[parity][col];
+                        if (m < a.M) a.out[at + m] = MODE == kFp8Dense ? acc[0][j][i] : wt * acc[0][j][i];
+                        if (m + 128 < a.M) a.out[at + m + 128] = MODE == kFp8Dense ? acc[1][j][i] : wt * acc[1][j][i];
+                    }
+                }
+        }
+    } else if (warp >= 4) {
+        // ---- rows of the pairs and their scales: four rows x 128 columns an instruction; a stage is announced two stages later, so that three are under way
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(gg::kRegRows));
+        constexpr int kGroups = NT / 16;                 // of four rows, this warp's
+        const uint32_t w = warp - 4, rr = lane >> 3, ck = lane & 7u;
+        uint32_t blk = 0;
+        auto announce = [&](uint32_t i) {
+            umma::fence_smem_to_async();
+            __syncwarp();
+            if (lane == 0) { mbar_arrive(bar_full + 8 * (i % T::kStages)); mbar_arrive(bar_sfull + 8 * (i % gg::kScales)); }
+        };
+        bool out = false;
+        for (uint32_t u = u_first; u < u_end && !out; ++u) {
+            const GroupUnit g = unit_of(u, live_i);
+            auto row_of = [&](uint32_t col) -> uint32_t {
+                uint64_t o;
+                float wt;
+                const uint32_t r = fp8_row<MODE>(a, g.p0 + min(col, g.n - 1), o, wt);   // (past the end the last one again: nobody looks at those columns)
+                return r == kFp8NoRow ? 0u : r;
+            };
+            const uint8_t* src[kGroups];
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) src[i] = a.xq + (uint64_t)row_of(16 * i + 4 * w + rr) * a.K + ck * 16u;
+            const uint32_t sc_col = w * 32 + lane;       // of the scales this lane brings
+            const float* sc_src = a.x_scale + (uint64_t)row_of(min(sc_col, (uint32_t)NT - 1)) * KB;
+            for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
+                const uint32_t s = blk % T::kStages, slot = blk % gg::kScales;
+                const bool there = kb * 128u + ck * 16u < a.K;
+                if (blk >= T::kStages) wait_bar(bar_empty + 8 * s, (blk / T::kStages - 1) & 1u);
+                if (blk >= gg::kScales) wait_bar(bar_sfree + 8 * slot, (blk / gg::kScales - 1) & 1u);
+                if (__any_sync(0xFFFFFFFFu, waits.out)) { out = true; break; }
+                const uint32_t dst = base + s * T::kStage + 32768u;
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i)
+                    if (16u * i < g.n)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + umma::sw128_chunk(16 * i + 4 * w + rr, ck)), "l"(there ? src[i] + kb * 128u : a.xq),
+                                     "r"(there ? 16u : 0u) : "memory");
+                if (sc_col < (uint32_t)NT)
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(base + T::kScale0 + (slot * NT + sc_col) * 4u), "l"(sc_src + kb) : "memory");
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (blk >= 2) {
+                    asm volatile("cp.async.wait_group 2;" ::: "memory");
+                    announce(blk - 2);
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (!out)
+            for (uint32_t i = blk > 2 ? blk - 2 : 0; i < blk; ++i) announce(i);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(gg::kRegAux));
+        if (warp == 0) {
+            // ---- weights
+            uint32_t blk = 0;
+            bool out = false;
+            for (uint32_t u = u_first; u < u_end && !out; ++u) {
+                const GroupUnit g = unit_of(u, live_i);
+                const uint32_t r0 = g.e * a.M + g.m0, r1 = kGateUp ? r0 : r0 + 128;
+                for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
+                    const uint32_t s = blk % T::kStages, dst = base + s * T::kStage, full = bar_full + 8 * s;
+                    if (blk >= T::kStages) wait_bar(bar_empty + 8 * s, (blk / T::kStages - 1) & 1u);
+                    if (__any_sync(0xFFFFFFFFu, waits.out)) { out = true; break; }   // a barrier that still counts bytes takes no second arrival
+                    if (lane == 0) {
+                        mbar_expect_tx(full, 32768u);
+                        tma_tile<1>(dst, &map0, kb * 128u, r0, full);
+                        tma_tile<1>(dst + 16384u, kGateUp ? &map1 : &map0, kb * 128u, r1, full);
+                    }
+                    __syncwarp();
+                }
+            }
+            for (uint32_t i = blk > T::kStages ? blk - T::kStages : 0; i < blk && !out; ++i) wait_bar(bar_empty + 8 * (i % T::kStages), (i / T::kStages) & 1u);
+        } else if (warp == 1) {
+            // ---- MMAs
+            const bool leader = umma::elect_one();
+            const uint64_t da0 = umma::smem_desc(base);
+            uint32_t s = 0, full_parity = 0, set = 0, free_parity = 1;
+            uint64_t da = da0;
+            for (uint32_t u = u_first; u < u_end; ++u) {
+                const GroupUnit g = unit_of(u, live_i);
+                const uint32_t idesc = instr_desc_e4m3(128, (g.n + 15u) & ~15u);
+                for (uint32_t kb = 0; kb < KB; ++kb) {
+                    wait_bar(bar_full + 8 * s, full_parity);
+                    wait_bar(bar_free + 8 * set, free_parity);
+                    umma::fence_after_sync();
+                    if (leader) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            mma_e4m3_ss<1>(tmem + set * T::kSetCols, da + 2 * j, da + 2048 + 2 * j, idesc, j != 0);
+                            mma_e4m3_ss<1>(tmem + set * T::kSetCols + NT, da + 1024 + 2 * j, da + 2048 + 2 * j, idesc, j != 0);
+                        }
+                        umma::commit(bar_set + 8 * set);
+                        umma::commit(bar_empty + 8 * s);
+                    }
+                    __syncwarp();
+                    da += T::kStage / 16;
+                    if (++s == T::kStages) { s = 0; da = da0; full_parity ^= 1u; }
+                    if (++set == T::kSets) { set = 0; free_parity ^= 1u; }
+                }
+            }
+        }
+    }
+    umma::fence_before_sync();
+    const int any_timed_out = __syncthreads_or(waits.out ? 1 : 0);
+    if (any_timed_out) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies and MMAs still under way end long before this does
+    if (warp == 2) umma::tmem_dealloc(tmem, 512);
+    if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
+}
+
 // tensor map over E4M3 rows [rows][K]: boxes of `box` rows x 128 columns, 128-byte swizzle, zeros outside
 bool fp8_map(CUtensorMap* map, const void* p, uint64_t rows, uint32_t K, uint32_t box) {
     typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -334,20 +650,20 @@ bool fp8_map(CUtensorMap* map, const void* p, uint64_t rows, uint32_t K, uint32_
 }
 
 // The register split needs what the launch bounds promise: less would leave the warps that ask for more waiting for good.
-template <auto Kernel>
+template <auto Kernel, int Want>
 cudaError_t check_registers() {
     static const int regs = [] {
         cudaFuncAttributes f{};
         return cudaFuncGetAttributes(&f, Kernel) == cudaSuccess ? f.numRegs : 0;
     }();
-    return regs >= tg::kRegLaunch ? cudaSuccess : cudaErrorInvalidKernelImage;
+    return regs >= Want ? cudaSuccess : cudaErrorInvalidKernelImage;
 }
 
 template <int CG>
 cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     using T = tg::Tile<CG>;
     if (const cudaError_t e = allow_dynamic_smem<fp8_wide_kernel<CG>>((int)T::kSmem)) return e;
-    if (const cudaError_t e = check_registers<fp8_wide_kernel<CG>>()) return e;
+    if (const cudaError_t e = check_registers<fp8_wide_kernel<CG>, tg::kRegLaunch>()) return e;
     CUtensorMap xm, wm;
     if (!fp8_map(&xm, a.xq, a.n, a.K, 128) || !fp8_map(&wm, a.w[0], a.M, a.K, T::kRowsW)) return cudaErrorInvalidValue;
     WideArgs w{};
@@ -372,10 +688,44 @@ cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
+template <int MODE, int NT>
+cudaError_t group_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
+    using T = gg::Tile<NT>;
+    constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    if (const cudaError_t e = allow_dynamic_smem<fp8_group_kernel<MODE, NT>>((int)T::kSmem)) return e;
+    if (const cudaError_t e = check_registers<fp8_group_kernel<MODE, NT>, gg::kRegLaunch>()) return e;
+    const uint64_t rows = (uint64_t)(kGrouped ? a.n_experts : 1u) * a.M;
+    CUtensorMap m0, m1;
+    if (rows > 0x7FFFFFFFu || !fp8_map(&m0, a.w[0], rows, a.K, 128) || !fp8_map(&m1, kGateUp ? a.w[1] : a.w[0], rows, a.K, 128)) return cudaErrorInvalidValue;
+    // blocks: as many as there can be units
+    const uint64_t per = kGateUp ? (a.M + 127) / 128 : (a.M + 255) / 256, pairs = kGrouped ? (uint64_t)a.n * a.n_used : a.n;
+    const uint64_t runs = kGrouped ? (pairs < a.n_experts ? pairs : pairs / NT + a.n_experts) : (pairs + NT - 1) / NT, units = per * runs;
+    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_group_kernel<MODE, NT>, dim3((uint32_t)(units < n_sms ? units : n_sms)), dim3(gg::kThreads), T::kSmem, a, m0, m1);
+    L.count();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int MODE>
+cudaError_t group_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
+    constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    const uint64_t mean = kGrouped ? (uint64_t)a.n * a.n_used / a.n_experts : a.n;
+    return mean > 24 ? group_launch<MODE, 128>(L, a, n_sms) : group_launch<MODE, 32>(L, a, n_sms);
+}
+
 }  // namespace
 
 cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) {
-    if (mode == kFp8Dense && a.n > 64 && a.K >= 128 && a.M >= 16) return a.n > 256 ? wide_launch<2>(L, a, n_sms) : wide_launch<1>(L, a, n_sms);
+    if (a.n == 0 || a.M == 0) return cudaSuccess;
+    if (a.K >= 128) switch (mode) {
+        case kFp8Dense:
+            if (a.n > 256) return wide_launch<2>(L, a, n_sms);
+            if (a.n > 16) return group_any<kFp8Dense>(L, a, n_sms);
+            break;
+        case kFp8GateUp: return group_any<kFp8GateUp>(L, a, n_sms);
+        case kFp8Down: return group_any<kFp8Down>(L, a, n_sms);
+        case kFp8SharedGateUp: if (a.n > 16) return group_any<kFp8SharedGateUp>(L, a, n_sms); break;
+        case kFp8SharedDown: if (a.n > 16) return group_any<kFp8SharedDown>(L, a, n_sms); break;
+    }
     return launch_fp8_rows(L, mode, a, n_sms);
 }
 
