@@ -7,10 +7,10 @@ namespace qkm {
 // ---- quantiser: f32 rows -> E4M3 with a power of two for each 128 columns -------------------------------------------------------
 // The scale is the smallest power of two that keeps the block's largest finite magnitude at or below 448 = 1.75 * 2^8, E4M3's largest:
 // dividing by it is exact, so an element is rounded once, by at most 2^-4 of itself (2^-10 of the scale below 2^-6 of it).
-// A warp takes a block of 128 columns, a lane four of them.
+// A warp takes a block of 128 columns, a lane four of them; of many blocks, four at a time, so that 2 KB a warp are under way.
 namespace {
 
-constexpr int kQuantThreads = 256;
+constexpr int kQuantThreads = 256, kQuantWarps = kQuantThreads / 32;
 
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     uint16_t lo, hi;
@@ -19,32 +19,49 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
+// BLOCKS consecutive blocks a warp; the matrix is one run of blocks where K is a multiple of 128 (WHOLE)
+template <int BLOCKS, bool WHOLE>
 __global__ void __launch_bounds__(kQuantThreads)
 fp8_quantize_kernel(const float* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scale, uint64_t n_blocks, uint32_t K, uint32_t KB) {
     const uint32_t lane = threadIdx.x & 31u;
-    const uint64_t b = (uint64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
+    const uint64_t b0 = ((uint64_t)blockIdx.x * kQuantWarps + (threadIdx.x >> 5)) * BLOCKS;
     pdl_trigger();
     pdl_wait();
-    if (b >= n_blocks) return;
-    const uint64_t row = b / KB;
-    const uint32_t col = (uint32_t)(b - row * KB) * 128u + lane * 4u;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (col < K) v = *reinterpret_cast<const float4*>(x + row * K + col);
-    float* e = &v.x;
-    uint32_t most = 0;
+    float4 v[BLOCKS];
+    uint64_t at[BLOCKS];
+    bool in[BLOCKS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t m = __float_as_uint(e[i]) & 0x7FFFFFFFu;
-        if (m < 0x7F800000u) most = max(most, m);
-        else e[i] = __uint_as_float(0x7FC00000u);          // E4M3 has no infinity: what is not finite becomes NaN
+    for (int i = 0; i < BLOCKS; ++i) {
+        const uint64_t b = b0 + i;
+        if (WHOLE) {
+            at[i] = b * 128u + lane * 4u;
+            in[i] = b < n_blocks;
+        } else {
+            const uint64_t row = b / KB;
+            const uint32_t col = (uint32_t)(b - row * KB) * 128u + lane * 4u;
+            at[i] = row * K + col;
+            in[i] = b < n_blocks && col < K;
+        }
+        v[i] = in[i] ? __ldcs(reinterpret_cast<const float4*>(x + at[i])) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    most = __reduce_max_sync(0xFFFFFFFFu, most);
-    // 1.75 * 2^E <= 448 * 2^(E - 8): the exponent moves up one where the mantissa is above 1.75
-    const uint32_t up = (most + 0x1FFFFFu) >> 23;
-    const uint32_t eb = most == 0 ? 127u : up > 9u ? up - 8u : 1u;
-    const float inv = __uint_as_float((254u - eb) << 23);
-    if (col < K) *reinterpret_cast<uint32_t*>(q + row * K + col) = e4m3x4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-    if (lane == 0) scale[b] = __uint_as_float(eb << 23);
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+        float* e = &v[i].x;
+        uint32_t most = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t m = __float_as_uint(e[j]) & 0x7FFFFFFFu;
+            if (m < 0x7F800000u) most = max(most, m);
+            else e[j] = __uint_as_float(0x7FC00000u);          // E4M3 has no infinity: what is not finite becomes NaN
+        }
+        most = __reduce_max_sync(0xFFFFFFFFu, most);
+        // 1.75 * 2^E <= 448 * 2^(E - 8): the exponent moves up one where the mantissa is above 1.75
+        const uint32_t up = (most + 0x1FFFFFu) >> 23;
+        const uint32_t eb = most == 0 ? 127u : up > 9u ? up - 8u : 1u;
+        const float inv = __uint_as_float((254u - eb) << 23);
+        if (in[i]) *reinterpret_cast<uint32_t*>(q + at[i]) = e4m3x4(e[0] * inv, e[1] * inv, e[2] * inv, e[3] * inv);
+        if (lane == 0 && b0 + i < n_blocks) scale[b0 + i] = __uint_as_float(eb << 23);
+    }
 }
 
 }  // namespace
@@ -52,9 +69,17 @@ fp8_quantize_kernel(const float* __restrict__ x, uint8_t* __restrict__ q, float*
 cudaError_t launch_fp8_quantize(const Launch& L, const float* x, uint32_t n, uint32_t K, void* q, float* scale) {
     if (n == 0) return cudaSuccess;
     const uint32_t KB = (K + 127) / 128;
-    const uint64_t blocks = (uint64_t)n * KB, grid = (blocks + kQuantThreads / 32 - 1) / (kQuantThreads / 32);
-    if (grid > 0x7FFFFFFFu) return cudaErrorInvalidValue;
-    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_quantize_kernel, dim3((uint32_t)grid), dim3(kQuantThreads), 0, x, (uint8_t*)q, scale, blocks, K, KB);
+    const uint64_t blocks = (uint64_t)n * KB;
+    auto go = [&](auto kernel, uint32_t per_warp) {
+        const uint64_t grid = (blocks + (uint64_t)kQuantWarps * per_warp - 1) / ((uint64_t)kQuantWarps * per_warp);
+        if (grid > 0x7FFFFFFFu) return cudaErrorInvalidValue;
+        return launch_kernel(Launch{L.stream, nullptr, true}, kernel, dim3((uint32_t)grid), dim3(kQuantThreads), 0, x, (uint8_t*)q, scale, blocks, K, KB);
+    };
+    // few blocks: as many warps as there are
+    cudaError_t e;
+    if (K % 128 == 0) e = blocks <= 8192 ? go(fp8_quantize_kernel<1, true>, 1) : go(fp8_quantize_kernel<4, true>, 4);
+    else e = blocks <= 8192 ? go(fp8_quantize_kernel<1, false>, 1) : go(fp8_quantize_kernel<4, false>, 4);
+    if (e == cudaErrorInvalidValue) return e;
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();
 }
