@@ -29,19 +29,33 @@ struct Fp8Args {
 
 __device__ __forceinline__ uint32_t fp8_blocks(uint32_t v) { return (v + 127u) / 128u; }
 
-// pair (or row) number p of expert e's run -> row of xq; kFp8NoRow where a list names a token or slot that there is none of
+// Entry of a list of pairs (of the shared expert and of a dense product: row number) -> row of xq and of the results; kFp8NoRow where it names a
+// token or slot that there is none of
+struct Fp8Place { uint32_t row; uint64_t out; };
+template <int MODE>
+__device__ __forceinline__ Fp8Place fp8_place(const Fp8Args& a, uint32_t entry) {
+    if (MODE == kFp8Dense) return {entry, entry};
+    if (MODE == kFp8SharedGateUp) return {entry, (uint64_t)entry * (a.n_used + 1) + a.n_used};
+    if (MODE == kFp8SharedDown) return {entry * (a.n_used + 1) + a.n_used, entry};
+    const uint32_t t = entry >> 4, s = entry & 15u;
+    if (t >= a.n || s >= a.n_used) return {kFp8NoRow, 0};
+    if (MODE == kFp8GateUp) return {t, (uint64_t)t * (a.n_used + 1) + s};
+    return {t * (a.n_used + 1) + s, (uint64_t)t * a.n_used + s};
+}
+// routing weight of an entry that has a place
+template <int MODE>
+__device__ __forceinline__ float fp8_weight(const Fp8Args& a, uint32_t entry) {
+    if (MODE == kFp8SharedDown) return a.sel[entry].w_shared;
+    if (MODE == kFp8Down) return a.sel[entry >> 4].w[entry & 15u];
+    return 1.f;
+}
 template <int MODE>
 __device__ __forceinline__ uint32_t fp8_row(const Fp8Args& a, uint32_t p, uint64_t& out_row, float& weight) {
-    weight = 1.f;
-    if (MODE == kFp8Dense) { out_row = p; return p; }
-    if (MODE == kFp8SharedGateUp) { out_row = (uint64_t)p * (a.n_used + 1) + a.n_used; return p; }
-    if (MODE == kFp8SharedDown) { out_row = p; weight = a.sel[p].w_shared; return p * (a.n_used + 1) + a.n_used; }
-    const uint32_t pr = a.pairs[p], t = pr >> 4, s = pr & 15u;
-    if (t >= a.n || s >= a.n_used) { out_row = 0; return kFp8NoRow; }
-    if (MODE == kFp8GateUp) { out_row = (uint64_t)t * (a.n_used + 1) + s; return t; }
-    out_row = (uint64_t)t * a.n_used + s;
-    weight = a.sel[t].w[s];
-    return t * (a.n_used + 1) + s;
+    const uint32_t entry = MODE == kFp8GateUp || MODE == kFp8Down ? a.pairs[p] : p;
+    const Fp8Place r = fp8_place<MODE>(a, entry);
+    out_row = r.out;
+    weight = r.row == kFp8NoRow ? 0.f : fp8_weight<MODE>(a, entry);
+    return r.row;
 }
 // expert e's run of the list of pairs, whatever the offsets hold inside the list
 __device__ __forceinline__ void fp8_run(const Fp8Args& a, uint32_t e, uint32_t& p0, uint32_t& p1) {

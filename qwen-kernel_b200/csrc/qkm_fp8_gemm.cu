@@ -324,17 +324,17 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
 // column block beside them; the eight warps that scale and add take the row scales from shared memory.
 namespace gg {
 constexpr int kThreads = 512;                    // warps: 0 weights, 1 MMAs, 2 tensor memory, 4 - 7 rows, 8 - 15 scale and add
-constexpr int kRegAux = 40, kRegRows = 56, kRegAdd = 208;
+constexpr int kRegAux = 40, kRegRows = 72, kRegAdd = 200;
 constexpr int kRegLaunch = 128;
 static_assert(128 * (kRegAux + kRegRows) + 256 * kRegAdd <= kThreads * kRegLaunch, "the shares must not exceed the launch's registers");
-constexpr uint32_t kMaxExperts = 512, kScales = 8;
+constexpr uint32_t kMaxExperts = 512, kScales = 8, kMeta = 4;   // scale slots; units whose columns' destinations are kept
 template <int NT> struct Tile {
     static constexpr uint32_t kStage = 2 * 16384 + NT * 128;
-    static constexpr uint32_t kStages = NT > 64 ? 4 : 6;
+    static constexpr uint32_t kStages = NT > 64 ? 4 : 5;
     static constexpr uint32_t kSets = NT > 64 ? 2 : 4;                 // of 2 NT columns; fewer than the scale slots less the stages
     static constexpr uint32_t kSetCols = 512 / kSets;
-    static constexpr uint32_t kScale0 = kStages * kStage;              // [kScales][NT] f32
-    static constexpr uint32_t kSmem = kScale0 + kScales * NT * 4 + 1024;
+    static constexpr uint32_t kScale0 = kStages * kStage;              // [kScales][2][NT] f32: row scale times either matrix's block scale
+    static constexpr uint32_t kSmem = kScale0 + kScales * NT * 8 + 1024;
     static constexpr int kChunk = NT / 4 < 32 ? NT / 4 : 32;           // columns of a load
     static constexpr int kChunks = NT / 2 / kChunk;                    // loads a warp and matrix
 };
@@ -354,24 +354,22 @@ template <int N> __device__ __forceinline__ void tmem_done(float (&a)[N], float 
 #pragma unroll
     for (int i = 0; i < N; ++i) asm volatile("" : "+f"(a[i]), "+f"(b[i]));
 }
-// acc[0..1] += v[0..1] * (x[0..1] * w)
-__device__ __forceinline__ void add2(float& a0, float& a1, float v0, float v1, float x0, float x1, uint64_t w2) {
-    asm("{\n"
-        ".reg .b64 v, c, x;\n"
-        "mov.b64 v, {%2, %3};\n"
-        "mov.b64 c, {%0, %1};\n"
-        "mov.b64 x, {%4, %5};\n"
-        "mul.rn.f32x2 x, x, %6;\n"
-        "fma.rn.f32x2 c, v, x, c;\n"
-        "mov.b64 {%0, %1}, c;\n"
-        "}\n"
-        : "+f"(a0), "+f"(a1) : "f"(v0), "f"(v1), "f"(x0), "f"(x1), "l"(w2));
+// acc[0..3] += v[0..3] * x[0..3]
+__device__ __forceinline__ void add4(float* a, const float* v, const uint4& x) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2)
+        asm("{\n"
+            ".reg .b64 v, c, x;\n"
+            "mov.b64 v, {%2, %3};\n"
+            "mov.b64 c, {%0, %1};\n"
+            "mov.b64 x, {%4, %5};\n"
+            "fma.rn.f32x2 c, v, x, c;\n"
+            "mov.b64 {%0, %1}, c;\n"
+            "}\n"
+            : "+f"(a[i]), "+f"(a[i + 1]) : "f"(v[i]), "f"(v[i + 1]), "r"(i ? x.z : x.x), "r"(i ? x.w : x.y));
 }
-__device__ __forceinline__ uint64_t twice(float w) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(w));
-    return r;
-}
+// silu(g) * u with the fast division (2 ulp; 0 where e^-g passes 2^126, of a result below 2^-119 |u|)
+__device__ __forceinline__ float silu_times(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
 template <int MODE, int NT>
 __global__ void __launch_bounds__(gg::kThreads, 1)
@@ -380,20 +378,21 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
     static_assert(T::kStages + T::kSets <= gg::kScales + 2, "a scale slot comes back before its next use is due");
     extern __shared__ uint8_t smem_dyn[];
-    __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets + 2 * gg::kScales];
+    __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets + 2 * gg::kScales + gg::kMeta];
     __shared__ uint32_t s_tmem, s_scan[16][2], s_n_live, s_n_units;
     __shared__ uint32_t s_unit[kGrouped ? gg::kMaxExperts + 1 : 2], s_p0[kGrouped ? gg::kMaxExperts : 1], s_p1[kGrouped ? gg::kMaxExperts : 1];
     __shared__ uint16_t s_live[kGrouped ? gg::kMaxExperts : 1];
-    __shared__ uint64_t s_out[2][NT];                // where a column's results go, ~0: nowhere
-    __shared__ float s_wt[2][NT];
+    __shared__ uint64_t s_out[gg::kMeta][NT];        // per unit: where a column's results go, ~0: nowhere; its routing weight
+    __shared__ float s_wt[gg::kMeta][NT];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
     const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * T::kStages, bar_set = bar_empty + 8 * T::kStages, bar_free = bar_set + 8 * T::kSets;
-    const uint32_t bar_sfull = bar_free + 8 * T::kSets, bar_sfree = bar_sfull + 8 * gg::kScales;
+    const uint32_t bar_sfull = bar_free + 8 * T::kSets, bar_sfree = bar_sfull + 8 * gg::kScales, bar_meta = bar_sfree + 8 * gg::kScales;
     if (tid == 0) {
         for (uint32_t i = 0; i < T::kStages; ++i) { mbar_init(bar_full + 8 * i, 1 + 4); mbar_init(bar_empty + 8 * i, 1); }
         for (uint32_t i = 0; i < T::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, 8); }
         for (uint32_t i = 0; i < gg::kScales; ++i) { mbar_init(bar_sfull + 8 * i, 4); mbar_init(bar_sfree + 8 * i, 8); }
+        for (uint32_t i = 0; i < gg::kMeta; ++i) mbar_init(bar_meta + 8 * i, 8);
         mbar_fence_init();
     }
     if (warp == 2) { umma::tmem_alloc(smem_addr(&s_tmem), 512); umma::tmem_relinquish(); }
@@ -453,20 +452,10 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     if (warp >= 8) {
         // ---- scale and add
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(gg::kRegAdd));
-        const uint32_t q = warp & 3u, h = (warp - 8) >> 2, c = tid - 256;
-        uint32_t blk = 0, set = 0, set_parity = 0, parity = 0;
-        for (uint32_t u = u_first; u < u_end; ++u, parity ^= 1u) {
+        const uint32_t q = warp & 3u, h = (warp - 8) >> 2;
+        uint32_t blk = 0, set = 0, set_parity = 0, meta = 0;
+        for (uint32_t u = u_first; u < u_end; ++u, meta = (meta + 1) % gg::kMeta) {
             const GroupUnit g = unit_of(u, live_i);
-            if (c < g.n) {
-                uint64_t row;
-                float wt;
-                const uint32_t r = fp8_row<MODE>(a, g.p0 + c, row, wt);
-                s_out[parity][c] = r == kFp8NoRow ? ~0ull : row * a.M;
-                s_wt[parity][c] = wt;
-            }
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            const float* ws0 = a.w_scale[0] + ((uint64_t)g.e * MB + g.m0 / 128u) * KB;
-            const float* ws1 = kGateUp ? a.w_scale[1] + ((uint64_t)g.e * MB + g.m0 / 128u) * KB : ws0 + (g.m0 / 128u + 1 < MB ? KB : 0u);
             float acc[2][T::kChunks][T::kChunk];
 #pragma unroll
             for (int m = 0; m < 2; ++m)
@@ -474,15 +463,11 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                 for (int j = 0; j < T::kChunks; ++j)
 #pragma unroll
                     for (int i = 0; i < T::kChunk; ++i) acc[m][j][i] = 0.f;
-            float w0 = ws0[0], w1 = ws1[0];
             for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
-                const uint32_t slot = blk % gg::kScales, sc = base + T::kScale0 + slot * NT * 4, t = tmem + ((32 * q) << 16) + set * T::kSetCols;
-                const float wc0 = w0, wc1 = w1;
-                if (kb + 1 < KB) { w0 = ws0[kb + 1]; w1 = ws1[kb + 1]; }
+                const uint32_t slot = blk % gg::kScales, sc = base + T::kScale0 + slot * NT * 8, t = tmem + ((32 * q) << 16) + set * T::kSetCols;
                 wait_bar(lane == 1 ? bar_sfull + 8 * slot : bar_set + 8 * set, lane == 1 ? (blk / gg::kScales) & 1u : set_parity);   // two barriers in one poll
                 __syncwarp();
                 umma::fence_after_sync();
-                const uint64_t wa = twice(wc0), wb = twice(wc1);
 #pragma unroll
                 for (int j = 0; j < T::kChunks; ++j) {
                     const uint32_t col = (2 * j + h) * T::kChunk;
@@ -493,12 +478,8 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                     tmem_done(v0, v1);
 #pragma unroll
                     for (int i = 0; i < T::kChunk; i += 4) {
-                        const uint4 x = lds128(sc + 4 * (col + i));
-                        const float x0 = __uint_as_float(x.x), x1 = __uint_as_float(x.y), x2 = __uint_as_float(x.z), x3 = __uint_as_float(x.w);
-                        add2(acc[0][j][i], acc[0][j][i + 1], v0[i], v0[i + 1], x0, x1, wa);
-                        add2(acc[0][j][i + 2], acc[0][j][i + 3], v0[i + 2], v0[i + 3], x2, x3, wa);
-                        add2(acc[1][j][i], acc[1][j][i + 1], v1[i], v1[i + 1], x0, x1, wb);
-                        add2(acc[1][j][i + 2], acc[1][j][i + 3], v1[i + 2], v1[i + 3], x2, x3, wb);
+                        add4(&acc[0][j][i], &v0[i], lds128(sc + 4 * (col + i)));
+                        add4(&acc[1][j][i], &v1[i], lds128(sc + 4 * (NT + col + i)));
                     }
                 }
                 umma::fence_before_sync();
@@ -506,65 +487,93 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                 if (lane == 0) { mbar_arrive(bar_free + 8 * set); mbar_arrive(bar_sfree + 8 * slot); }
                 if (++set == T::kSets) { set = 0; set_parity ^= 1u; }
             }
-            if (__any_sync(0xFFFFFFFFu, waits.out)) continue;   // (on through the list: the other warps meet this one at the barrier above)
-            const uint32_t m = g.m0 + 32 * q + lane;
+            if (!__any_sync(0xFFFFFFFFu, waits.out)) {
+                const uint32_t m = g.m0 + 32 * q + lane;
+                const bool in0 = m < a.M, in1 = m + 128 < a.M;
 #pragma unroll
-            for (int j = 0; j < T::kChunks; ++j)
+                for (int j = 0; j < T::kChunks; ++j)
 #pragma unroll
-                for (int i = 0; i < T::kChunk; ++i) {
-                    const uint32_t col = (2 * j + h) * T::kChunk + i;
-                    if (col >= g.n) continue;
-                    const uint64_t at = s_out[parity][col];
-                    if (at == ~0ull) continue;
-                    if (kGateUp) {
-                        if (m < a.M) a.out[at + m] = swiglu(acc[0][j][i], acc[1][j][i]);
-                    } else {
-                        const float wt = MODE == kFp8Dense ? 1.f : s_wt[parity][col];
-                        if (m < a.M) a.out[at + m] = MODE == kFp8Dense ? acc[0][j][i] : wt * acc[0][j][i];
-                        if (m + 128 < a.M) a.out[at + m + 128] = MODE == kFp8Dense ? acc[1][j][i] : wt * acc[1][j][i];
+                    for (int i = 0; i < T::kChunk; ++i) {
+                        const uint32_t col = (2 * j + h) * T::kChunk + i;
+                        if (col >= g.n) continue;
+                        const uint64_t at = s_out[meta][col];
+                        if (at == ~0ull) continue;
+                        float* out = a.out + at + m;
+                        if (kGateUp) {
+                            if (in0) *out = silu_times(acc[0][j][i], acc[1][j][i]);
+                        } else {
+                            const float wt = MODE == kFp8Dense ? 1.f : s_wt[meta][col];
+                            if (in0) *out = MODE == kFp8Dense ? acc[0][j][i] : wt * acc[0][j][i];
+                            if (in1) out[128] = MODE == kFp8Dense ? acc[1][j][i] : wt * acc[1][j][i];
+                        }
                     }
-                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_meta + 8 * meta);
         }
     } else if (warp >= 4) {
-        // ---- rows of the pairs and their scales: four rows x 128 columns an instruction; a stage is announced two stages later, so that three are under way
+        // ---- rows of the pairs: four rows x 128 columns an instruction; a stage is announced two stages later, so that three are under way.  Beside them,
+        // a lane for each column: the scales, multiplied, and where the column's results go.  The list of the next unit's pairs is read a unit ahead.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(gg::kRegRows));
         constexpr int kGroups = NT / 16;                 // of four rows, this warp's
-        const uint32_t w = warp - 4, rr = lane >> 3, ck = lane & 7u;
-        uint32_t blk = 0;
+        const uint32_t w = warp - 4, rr = lane >> 3, ck = lane & 7u, mine = w * 32 + lane;
+        uint32_t blk = 0, unit = 0;
         auto announce = [&](uint32_t i) {
             umma::fence_smem_to_async();
             __syncwarp();
             if (lane == 0) { mbar_arrive(bar_full + 8 * (i % T::kStages)); mbar_arrive(bar_sfull + 8 * (i % gg::kScales)); }
         };
+        // entry of the list for a column, the last one past the end (nobody looks at those columns)
+        auto entry = [&](const GroupUnit& g, uint32_t col) -> uint32_t { const uint32_t p = g.p0 + min(col, g.n - 1); return kGrouped ? a.pairs[p] : p; };
+        GroupUnit g{};
+        uint32_t pr[kGroups], pr_mine = 0;
+        auto entries = [&](uint32_t u) {
+            g = unit_of(u, live_i);
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) pr[i] = entry(g, 16 * i + 4 * w + rr);
+            if (mine < (uint32_t)NT) pr_mine = entry(g, mine);
+        };
+        if (u_first < u_end) entries(u_first);
         bool out = false;
-        for (uint32_t u = u_first; u < u_end && !out; ++u) {
-            const GroupUnit g = unit_of(u, live_i);
-            auto row_of = [&](uint32_t col) -> uint32_t {
-                uint64_t o;
-                float wt;
-                const uint32_t r = fp8_row<MODE>(a, g.p0 + min(col, g.n - 1), o, wt);   // (past the end the last one again: nobody looks at those columns)
-                return r == kFp8NoRow ? 0u : r;
-            };
+        for (uint32_t u = u_first; u < u_end && !out; ++u, ++unit) {
+            const uint32_t n = g.n, meta = unit % gg::kMeta;
             const uint8_t* src[kGroups];
 #pragma unroll
-            for (int i = 0; i < kGroups; ++i) src[i] = a.xq + (uint64_t)row_of(16 * i + 4 * w + rr) * a.K + ck * 16u;
-            const uint32_t sc_col = w * 32 + lane;       // of the scales this lane brings
-            const float* sc_src = a.x_scale + (uint64_t)row_of(min(sc_col, (uint32_t)NT - 1)) * KB;
+            for (int i = 0; i < kGroups; ++i) {
+                const Fp8Place r = fp8_place<MODE>(a, pr[i]);
+                src[i] = a.xq + (uint64_t)(r.row == kFp8NoRow ? 0u : r.row) * a.K + ck * 16u;
+            }
+            const Fp8Place me = fp8_place<MODE>(a, pr_mine);
+            const float* xs = a.x_scale + (uint64_t)(me.row == kFp8NoRow ? 0u : me.row) * KB;
+            const float* ws0 = a.w_scale[0] + ((uint64_t)g.e * MB + g.m0 / 128u) * KB;
+            const float* ws1 = kGateUp ? a.w_scale[1] + ((uint64_t)g.e * MB + g.m0 / 128u) * KB : ws0 + (g.m0 / 128u + 1 < MB ? KB : 0u);
+            const float wt = me.row == kFp8NoRow || mine >= (uint32_t)NT ? 0.f : fp8_weight<MODE>(a, pr_mine);
+            float x0 = xs[0], wa0 = ws0[0], wb0 = ws1[0], x1 = KB > 1 ? xs[1] : 0.f, wa1 = KB > 1 ? ws0[1] : 0.f, wb1 = KB > 1 ? ws1[1] : 0.f;
+            if (unit >= gg::kMeta) wait_bar(bar_meta + 8 * meta, (unit / gg::kMeta - 1) & 1u);
+            if (mine < (uint32_t)NT) s_out[meta][mine] = mine >= n || me.row == kFp8NoRow ? ~0ull : me.out * a.M;
+            if (u + 1 < u_end) entries(u + 1);
             for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
                 const uint32_t s = blk % T::kStages, slot = blk % gg::kScales;
                 const bool there = kb * 128u + ck * 16u < a.K;
+                const float xc = x0, wac = wa0, wbc = wb0;
+                x0 = x1; wa0 = wa1; wb0 = wb1;
+                if (kb + 2 < KB) { x1 = xs[kb + 2]; wa1 = ws0[kb + 2]; wb1 = ws1[kb + 2]; }
                 if (blk >= T::kStages) wait_bar(bar_empty + 8 * s, (blk / T::kStages - 1) & 1u);
                 if (blk >= gg::kScales) wait_bar(bar_sfree + 8 * slot, (blk / gg::kScales - 1) & 1u);
                 if (__any_sync(0xFFFFFFFFu, waits.out)) { out = true; break; }
                 const uint32_t dst = base + s * T::kStage + 32768u;
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i)
-                    if (16u * i < g.n)
+                    if (16u * i < n)
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + umma::sw128_chunk(16 * i + 4 * w + rr, ck)), "l"(there ? src[i] + kb * 128u : a.xq),
                                      "r"(there ? 16u : 0u) : "memory");
-                if (sc_col < (uint32_t)NT)
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(base + T::kScale0 + (slot * NT + sc_col) * 4u), "l"(sc_src + kb) : "memory");
                 asm volatile("cp.async.commit_group;" ::: "memory");
+                if (mine < (uint32_t)NT) {
+                    const uint32_t sc = base + T::kScale0 + (slot * 2 * NT + mine) * 4u;
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc), "f"(xc * wac) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc + NT * 4u), "f"(xc * wbc) : "memory");
+                    if (kb + 1 == KB) s_wt[meta][mine] = wt;
+                }
                 if (blk >= 2) {
                     asm volatile("cp.async.wait_group 2;" ::: "memory");
                     announce(blk - 2);
