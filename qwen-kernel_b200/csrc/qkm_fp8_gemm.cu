@@ -342,11 +342,73 @@ template <int NT> struct Tile {
 
 struct GroupUnit { uint32_t e, m0, p0, n; };     // expert, first weight row, first pair, pairs
 
+// The units of a product: experts that have pairs (of a dense product or the shared expert the one matrix), their runs of pairs cut into parts of PART,
+// every part with all row units of the expert; the parts of a row unit next to one another.
+template <int MODE, int PART>
+struct UnitList {
+    static constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    static constexpr uint32_t kMax = kGrouped ? gg::kMaxExperts : 1u;
+    uint32_t unit[kMax + 1], p0[kMax], p1[kMax];     // per live expert: first unit, run
+    uint32_t scan[16][2], n_live, n_units;
+    uint16_t expert[kMax];
+
+    // by all threads of the block (256 or more; two experts each); __syncthreads behind it
+    __device__ __forceinline__ void make(const Fp8Args& a) {
+        const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, row_units = kGateUp ? (a.M + 127) / 128 : (a.M + 255) / 256;
+        uint32_t q0[2] = {}, q1[2] = {}, units[2], c = 0, v = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t e = 2 * tid + i;
+            if (kGrouped) { if (e < a.n_experts) fp8_run(a, e, q0[i], q1[i]); }
+            else if (e == 0) q1[i] = a.n;
+            units[i] = (q1[i] - q0[i] + PART - 1) / PART * row_units;
+            c += units[i] ? 1u : 0u;
+            v += units[i];
+        }
+        const uint32_t c_mine = c, v_mine = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t c1 = __shfl_up_sync(0xFFFFFFFFu, c, o), v1 = __shfl_up_sync(0xFFFFFFFFu, v, o);
+            if (lane >= (uint32_t)o) { c += c1; v += v1; }
+        }
+        if (lane == 31) { scan[warp][0] = c; scan[warp][1] = v; }
+        __syncthreads();
+        for (uint32_t w = 0; w < warp; ++w) { c += scan[w][0]; v += scan[w][1]; }
+        if (tid == blockDim.x - 1) { n_live = c; n_units = v; unit[c] = v; }
+        c -= c_mine; v -= v_mine;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (units[i]) {
+                expert[c] = (uint16_t)(2 * tid + i); p0[c] = q0[i]; p1[c] = q1[i]; unit[c] = v;
+                ++c;
+                v += units[i];
+            }
+    }
+    // position in the list of the expert that unit u belongs to
+    __device__ __forceinline__ uint32_t find(uint32_t u) const {
+        uint32_t i = 0;
+        if (kGrouped && u < n_units)
+            for (uint32_t step = kMax / 2; step; step >>= 1)
+                if (i + step < n_live && unit[i + step] <= u) i += step;
+        return i;
+    }
+    // unit u; i: its expert's position or an earlier one
+    __device__ __forceinline__ GroupUnit at(uint32_t u, uint32_t& i) const {
+        while (u >= unit[i + 1]) ++i;
+        const uint32_t run = p1[i] - p0[i], parts = (run + PART - 1) / PART, k = u - unit[i], ru = k / parts, part = k - ru * parts;
+        GroupUnit g;
+        g.e = kGrouped ? expert[i] : 0u;
+        g.m0 = ru * (kGateUp ? 128u : 256u);
+        g.p0 = p0[i] + part * PART;
+        g.n = min((uint32_t)PART, run - part * PART);
+        return g;
+    }
+};
+
 __device__ __forceinline__ void tmem_ld8f(uint32_t taddr, float (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_load(uint32_t t, float (&v)[32]) { tmem_ld32(t, v); }
 __device__ __forceinline__ void tmem_load(uint32_t t, float (&v)[8]) { tmem_ld8f(t, v); }
 // waits for the loads, whose registers are used behind it
 template <int N> __device__ __forceinline__ void tmem_done(float (&a)[N], float (&b)[N]) {
@@ -379,9 +441,8 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     static_assert(T::kStages + T::kSets <= gg::kScales + 2, "a scale slot comes back before its next use is due");
     extern __shared__ uint8_t smem_dyn[];
     __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets + 2 * gg::kScales + gg::kMeta];
-    __shared__ uint32_t s_tmem, s_scan[16][2], s_n_live, s_n_units;
-    __shared__ uint32_t s_unit[kGrouped ? gg::kMaxExperts + 1 : 2], s_p0[kGrouped ? gg::kMaxExperts : 1], s_p1[kGrouped ? gg::kMaxExperts : 1];
-    __shared__ uint16_t s_live[kGrouped ? gg::kMaxExperts : 1];
+    __shared__ uint32_t s_tmem;
+    __shared__ UnitList<MODE, NT> s_list;
     __shared__ uint64_t s_out[gg::kMeta][NT];        // per unit: where a column's results go, ~0: nowhere; its routing weight
     __shared__ float s_wt[gg::kMeta][NT];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -399,46 +460,14 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     umma::fence_before_sync();
     pdl_trigger();
     pdl_wait();
-    const uint32_t KB = fp8_blocks(a.K), MB = fp8_blocks(a.M), row_units = kGateUp ? (a.M + 127) / 128 : (a.M + 255) / 256;
-    // the list of units: experts that have pairs, their first unit and their run
-    {
-        uint32_t p0 = 0, p1 = 0;
-        if (kGrouped) { if (tid < a.n_experts) fp8_run(a, tid, p0, p1); }
-        else if (tid == 0) p1 = a.n;
-        const uint32_t live = p1 > p0 ? 1u : 0u, mine = (p1 - p0 + NT - 1) / NT * row_units;
-        uint32_t c = live, v = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t c1 = __shfl_up_sync(0xFFFFFFFFu, c, o), v1 = __shfl_up_sync(0xFFFFFFFFu, v, o);
-            if (lane >= (uint32_t)o) { c += c1; v += v1; }
-        }
-        if (lane == 31) { s_scan[warp][0] = c; s_scan[warp][1] = v; }
-        __syncthreads();
-        for (uint32_t w = 0; w < warp; ++w) { c += s_scan[w][0]; v += s_scan[w][1]; }
-        if (live) {
-            const uint32_t i = c - 1;
-            s_live[i] = (uint16_t)tid; s_p0[i] = p0; s_p1[i] = p1; s_unit[i] = v - mine; s_unit[i + 1] = v;   // (the next one writes the same there)
-        }
-        if (tid == gg::kThreads - 1) { s_n_live = c; s_n_units = v; }
-    }
+    const uint32_t KB = fp8_blocks(a.K), MB = fp8_blocks(a.M);
+    s_list.make(a);
     __syncthreads();
     umma::fence_after_sync();
-    const uint32_t tmem = s_tmem, n_units = s_n_units;
+    const uint32_t tmem = s_tmem, n_units = s_list.n_units;
     const uint32_t u_first = (uint32_t)((uint64_t)n_units * blockIdx.x / gridDim.x), u_end = (uint32_t)((uint64_t)n_units * (blockIdx.x + 1) / gridDim.x);
-    uint32_t live_i = 0;
-    if (kGrouped && u_first < u_end)   // the expert of the first unit, by halves
-        for (uint32_t step = gg::kMaxExperts / 2; step; step >>= 1)
-            if (live_i + step < s_n_live && s_unit[live_i + step] <= u_first) live_i += step;
-    auto unit_of = [&](uint32_t u, uint32_t& i) -> GroupUnit {
-        while (u >= s_unit[i + 1]) ++i;
-        const uint32_t run = s_p1[i] - s_p0[i], parts = (run + NT - 1) / NT, at = u - s_unit[i], ru = at / parts, part = at - ru * parts;
-        GroupUnit g;
-        g.e = kGrouped ? s_live[i] : 0u;
-        g.m0 = ru * (kGateUp ? 128u : 256u);
-        g.p0 = s_p0[i] + part * NT;
-        g.n = min((uint32_t)NT, run - part * NT);
-        return g;
-    };
+    uint32_t live_i = s_list.find(u_first);
+    auto unit_of = [&](uint32_t u, uint32_t& i) -> GroupUnit { return s_list.at(u, i); };
     Waits waits;
     auto wait_bar = [&](uint32_t b, uint32_t parity) {
         waits.wait([&] {
@@ -642,6 +671,248 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
 }
 
+// ---- the same with the pairs as lanes, for experts of many pairs ------------------------------------------------------------------------
+// A unit is up to 128 pairs (the MMAs' rows, a lane each) times 256 weight rows: the gate and the up rows of a 128-row tile, or two tiles of one matrix.  What a
+// thread scales is then one row's, as in the dense kernel: an FMA for two elements and nothing else.  (With the weight rows as lanes the scales of 128 columns came from shared
+// memory and the sums went out by single words: gate/up of 4096 tokens 281 us, down 243.)
+namespace pg {
+constexpr int kThreads = 384;                    // warps: 0 weights, 1 MMAs, 2 - 3 rows (2: tensor memory), 4 - 11 scale and add
+constexpr int kRegAux = 56, kRegAdd = 224;
+constexpr int kRegLaunch = 168;
+static_assert(128 * kRegAux + 256 * kRegAdd <= kThreads * kRegLaunch, "the shares must not exceed the launch's registers");
+constexpr uint32_t kStage = 3 * 16384, kStages = 4, kPut = kStages * kStage, kSmem = kPut + 8 * 2048 + 1024;   // 2 KB a warp on the way to coalesced stores
+}  // namespace pg
+
+template <int MODE>
+__global__ void __launch_bounds__(pg::kThreads, 1)
+fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1) {
+    constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    extern __shared__ uint8_t smem_dyn[];
+    __shared__ __align__(8) unsigned long long s_bar[2 * pg::kStages + 4];
+    __shared__ uint32_t s_tmem;
+    __shared__ UnitList<MODE, 128> s_list;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
+    const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * pg::kStages, bar_set = bar_empty + 8 * pg::kStages, bar_free = bar_set + 16;
+    if (tid == 0) {
+        for (uint32_t i = 0; i < pg::kStages; ++i) { mbar_init(bar_full + 8 * i, 1 + 2); mbar_init(bar_empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < 2; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, 8); }
+        mbar_fence_init();
+    }
+    if (warp == 2) { umma::tmem_alloc(smem_addr(&s_tmem), 512); umma::tmem_relinquish(); }
+    umma::fence_before_sync();
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t KB = fp8_blocks(a.K), MB = fp8_blocks(a.M);
+    s_list.make(a);
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = s_tmem, n_units = s_list.n_units;
+    const uint32_t u_first = (uint32_t)((uint64_t)n_units * blockIdx.x / gridDim.x), u_end = (uint32_t)((uint64_t)n_units * (blockIdx.x + 1) / gridDim.x);
+    uint32_t live_i = s_list.find(u_first);
+    Waits waits;
+    auto wait_bar = [&](uint32_t b, uint32_t parity) {
+        waits.wait([&] {
+#pragma unroll 1
+            for (int i = 0; i < 64; ++i)
+                if (mbar_try_wait(b, parity)) return true;
+            return mbar_wait_timed(b, parity);
+        });
+    };
+    // entry of the list of pairs for a row of a unit, the last one past its end (nobody looks at those rows)
+    auto entry = [&](const GroupUnit& g, uint32_t row) -> uint32_t { const uint32_t p = g.p0 + min(row, g.n - 1); return kGrouped ? a.pairs[p] : p; };
+
+    if (warp >= 4) {
+        // ---- scale and add: TMEM lanes 32 q ..; of gate/up 64 columns of either matrix, else 128 columns of one tile
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(pg::kRegAdd));
+        const uint32_t q = warp & 3u, h = (warp - 4) >> 2, row = 32 * q + lane;
+        const uint32_t put = base + pg::kPut + (warp - 4) * 2048u;
+        const uint32_t c0 = kGateUp ? 64 * h : 128 * h, c1 = kGateUp ? 128 + 64 * h : 128 * h + 64;   // first columns of the two runs of 64
+        const uint32_t t0 = tmem + ((32 * q) << 16);
+        uint32_t blk = 0, next = 0;                          // next: this row's entry of the list, read a unit ahead
+        bool ready = false;
+        GroupUnit g{};
+        if (u_first < u_end) { g = s_list.at(u_first, live_i); next = entry(g, row); }
+        for (uint32_t u = u_first; u < u_end; ++u) {
+            const GroupUnit cur = g;
+            const uint32_t mine = next;
+            const Fp8Place me = fp8_place<MODE>(a, mine);
+            const float* xs = a.x_scale + (uint64_t)(me.row == kFp8NoRow ? 0u : me.row) * KB;
+            const float* ws0 = a.w_scale[0] + ((uint64_t)cur.e * MB + (kGateUp ? cur.m0 / 128u : min(cur.m0 / 128u + h, MB - 1))) * KB;
+            const float* ws1 = kGateUp ? a.w_scale[1] + ((uint64_t)cur.e * MB + cur.m0 / 128u) * KB : ws0;
+            float x0 = xs[0], wa0 = ws0[0], wb0 = ws1[0];
+            const float wt = me.row == kFp8NoRow ? 0.f : fp8_weight<MODE>(a, mine);
+            if (u + 1 < u_end) { g = s_list.at(u + 1, live_i); next = entry(g, row); }
+            float acc[2][64];
+#pragma unroll
+            for (int i = 0; i < 128; ++i) acc[i >> 6][i & 63] = 0.f;
+            const bool work = 32 * q < cur.n;                // some row of this warp's is there
+            for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
+                const uint32_t set = blk & 1u, t = t0 + set * 256u;
+                const float xc = x0, wac = wa0, wbc = wb0;
+                if (kb + 1 < KB) { x0 = xs[kb + 1]; wa0 = ws0[kb + 1]; wb0 = ws1[kb + 1]; }
+                if (!ready) wait_bar(bar_set + 8 * set, (blk >> 1) & 1u);
+                umma::fence_after_sync();
+                float v[32];
+                if (work) {
+                    const float s = xc * wac;
+#pragma unroll
+                    for (int c = 0; c < 3; ++c) {
+                        tmem_ld32(t + (c < 2 ? c0 + 32 * c : c1), v);
+                        tmem_ld_done(v);
+                        add_scaled(acc[c >> 1], 32 * (c & 1), v, c < 2 ? s : xc * (kGateUp ? wbc : wac));
+                    }
+                    tmem_ld32(t + c1 + 32, v);
+                    tmem_ld_done(v);
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_free + 8 * set);
+                ready = mbar_test(bar_set + 8 * (set ^ 1u), ((blk + 1) >> 1) & 1u);
+                if (work) add_scaled(acc[1], 32, v, xc * (kGateUp ? wbc : wac));
+            }
+            if (__any_sync(0xFFFFFFFFu, waits.out)) break;
+            if (!work) continue;
+            // 32 rows x 16 columns at a time through shared memory, four lanes a row for the stores
+            const uint64_t out0 = row >= cur.n || me.row == kFp8NoRow ? ~0ull : me.out * a.M;
+            const uint32_t m0 = cur.m0 + (kGateUp ? 64 * h : 128 * h);
+#pragma unroll
+            for (int c = 0; c < (kGateUp ? 4 : 8); ++c) {
+                float r[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    r[i] = kGateUp ? silu_times(acc[0][16 * c + i], acc[1][16 * c + i]) : MODE == kFp8Dense ? acc[c >> 2][16 * (c & 3) + i] : wt * acc[c >> 2][16 * (c & 3) + i];
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(put + lane * 64u + ((j ^ ((lane >> 1) & 3u)) << 4)), "f"(r[4 * j]), "f"(r[4 * j + 1]), "f"(r[4 * j + 2]),
+                                 "f"(r[4 * j + 3]) : "memory");
+                __syncwarp();
+                const uint32_t j = lane & 3u, m = m0 + 16 * c + 4 * j;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t rr = 8 * i + (lane >> 2);
+                    const uint4 o = lds128(put + rr * 64u + ((j ^ ((rr >> 1) & 3u)) << 4));
+                    const uint64_t at = __shfl_sync(0xFFFFFFFFu, out0, rr);
+                    if (at == ~0ull) continue;
+                    float* y = a.out + at + m;
+                    if (a.vec) {
+                        if (m < a.M) *reinterpret_cast<uint4*>(y) = o;
+                    } else {
+                        const uint32_t e[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (m + k < a.M) y[k] = __uint_as_float(e[k]);
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(pg::kRegAux));
+        if (warp >= 2) {
+            // ---- rows: four x 128 columns an instruction, every other four this warp's; a stage is announced two stages later, so that three are under way
+            const uint32_t w = warp - 2, rr = lane >> 3, ck = lane & 7u;
+            uint32_t blk = 0;
+            auto announce = [&](uint32_t i) {
+                umma::fence_smem_to_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_full + 8 * (i % pg::kStages));
+            };
+            GroupUnit g{};
+            uint32_t pr[2];                                  // entries of the warp's rows number lane and lane + 32, read a unit ahead; number i is row 8 (i / 4) + 4 w + i % 4
+            auto entries = [&](uint32_t u) {
+                g = s_list.at(u, live_i);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) pr[i] = entry(g, (lane + 32 * i) / 4 * 8 + 4 * w + (lane & 3u));
+            };
+            if (u_first < u_end) entries(u_first);
+            bool out = false;
+            for (uint32_t u = u_first; u < u_end && !out; ++u) {
+                const uint32_t n = g.n;
+                uint32_t mine[2];                            // their rows of xq
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const Fp8Place r = fp8_place<MODE>(a, pr[i]);
+                    mine[i] = r.row == kFp8NoRow ? 0u : r.row;
+                }
+                uint32_t rows[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) rows[i] = __shfl_sync(0xFFFFFFFFu, mine[i >> 3], (4 * i + rr) & 31u);
+                if (u + 1 < u_end) entries(u + 1);
+                for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
+                    const uint32_t s = blk % pg::kStages;
+                    const bool there = kb * 128u + ck * 16u < a.K;
+                    if (blk >= pg::kStages) wait_bar(bar_empty + 8 * s, (blk / pg::kStages - 1) & 1u);
+                    if (__any_sync(0xFFFFFFFFu, waits.out)) { out = true; break; }
+                    const uint32_t dst = base + s * pg::kStage;
+                    const uint8_t* src = a.xq + kb * 128u + ck * 16u;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (8u * i < n)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + umma::sw128_chunk(8 * i + 4 * w + rr, ck)), "l"(there ? src + (uint64_t)rows[i] * a.K : a.xq),
+                                         "r"(there ? 16u : 0u) : "memory");
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (blk >= 2) {
+                        asm volatile("cp.async.wait_group 2;" ::: "memory");
+                        announce(blk - 2);
+                    }
+                }
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (!out)
+                for (uint32_t i = blk > 2 ? blk - 2 : 0; i < blk; ++i) announce(i);
+        } else if (warp == 0) {
+            // ---- weights
+            uint32_t blk = 0;
+            bool out = false;
+            for (uint32_t u = u_first; u < u_end && !out; ++u) {
+                const GroupUnit g = s_list.at(u, live_i);
+                const uint32_t r0 = g.e * a.M + g.m0, r1 = kGateUp ? r0 : r0 + 128;
+                for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
+                    const uint32_t s = blk % pg::kStages, dst = base + s * pg::kStage + 16384u, full = bar_full + 8 * s;
+                    if (blk >= pg::kStages) wait_bar(bar_empty + 8 * s, (blk / pg::kStages - 1) & 1u);
+                    if (__any_sync(0xFFFFFFFFu, waits.out)) { out = true; break; }   // a barrier that still counts bytes takes no second arrival
+                    if (lane == 0) {
+                        mbar_expect_tx(full, 32768u);
+                        tma_tile<1>(dst, &map0, kb * 128u, r0, full);
+                        tma_tile<1>(dst + 16384u, kGateUp ? &map1 : &map0, kb * 128u, r1, full);
+                    }
+                    __syncwarp();
+                }
+            }
+            for (uint32_t i = blk > pg::kStages ? blk - pg::kStages : 0; i < blk && !out; ++i) wait_bar(bar_empty + 8 * (i % pg::kStages), (i / pg::kStages) & 1u);
+        } else {
+            // ---- MMAs
+            const bool leader = umma::elect_one();
+            const uint32_t idesc = instr_desc_e4m3(128, 256), steps = (u_end - u_first) * KB;
+            const uint64_t da0 = umma::smem_desc(base);
+            uint32_t s = 0, full_parity = 0, set = 0, free_parity = 1;
+            uint64_t da = da0;
+            for (uint32_t i = 0; i < steps; ++i) {
+                wait_bar(bar_full + 8 * s, full_parity);
+                wait_bar(bar_free + 8 * set, free_parity);
+                umma::fence_after_sync();
+                if (leader) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_e4m3_ss<1>(tmem + set * 256u, da + 2 * j, da + 1024 + 2 * j, idesc, j != 0);
+                    umma::commit(bar_set + 8 * set);
+                    umma::commit(bar_empty + 8 * s);
+                }
+                __syncwarp();
+                da += pg::kStage / 16;
+                if (++s == pg::kStages) { s = 0; da = da0; full_parity ^= 1u; }
+                set ^= 1u;
+                free_parity ^= set ^ 1u;
+            }
+        }
+    }
+    umma::fence_before_sync();
+    const int any_timed_out = __syncthreads_or(waits.out ? 1 : 0);
+    if (any_timed_out) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies and MMAs still under way end long before this does
+    if (warp == 2) umma::tmem_dealloc(tmem, 512);
+    if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
+}
+
 // tensor map over E4M3 rows [rows][K]: boxes of `box` rows x 128 columns, 128-byte swizzle, zeros outside
 bool fp8_map(CUtensorMap* map, const void* p, uint64_t rows, uint32_t K, uint32_t box) {
     typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -715,10 +986,27 @@ cudaError_t group_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
 }
 
 template <int MODE>
+cudaError_t pairs_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
+    constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    if (const cudaError_t e = allow_dynamic_smem<fp8_pairs_kernel<MODE>>((int)pg::kSmem)) return e;
+    if (const cudaError_t e = check_registers<fp8_pairs_kernel<MODE>, pg::kRegLaunch>()) return e;
+    const uint64_t rows = (uint64_t)(kGrouped ? a.n_experts : 1u) * a.M;
+    CUtensorMap m0, m1;
+    if (rows > 0x7FFFFFFFu || !fp8_map(&m0, a.w[0], rows, a.K, 128) || !fp8_map(&m1, kGateUp ? a.w[1] : a.w[0], rows, a.K, 128)) return cudaErrorInvalidValue;
+    Fp8Args b = a;
+    b.vec = a.M % 4 == 0 && ((uintptr_t)a.out & 15u) == 0;
+    const uint64_t per = kGateUp ? (a.M + 127) / 128 : (a.M + 255) / 256, pairs = kGrouped ? (uint64_t)a.n * a.n_used : a.n;
+    const uint64_t runs = kGrouped ? (pairs < a.n_experts ? pairs : pairs / 128 + a.n_experts) : (pairs + 127) / 128, units = per * runs;
+    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_pairs_kernel<MODE>, dim3((uint32_t)(units < n_sms ? units : n_sms)), dim3(pg::kThreads), pg::kSmem, b, m0, m1);
+    L.count();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int MODE>
 cudaError_t group_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
     const uint64_t mean = kGrouped ? (uint64_t)a.n * a.n_used / a.n_experts : a.n;
-    return mean > 24 ? group_launch<MODE, 128>(L, a, n_sms) : group_launch<MODE, 32>(L, a, n_sms);
+    return mean > 24 ? pairs_launch<MODE>(L, a, n_sms) : group_launch<MODE, 32>(L, a, n_sms);
 }
 
 }  // namespace
