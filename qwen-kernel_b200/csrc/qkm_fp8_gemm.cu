@@ -676,10 +676,11 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
 // thread scales is then one row's, as in the dense kernel: an FMA for two elements and nothing else.  (With the weight rows as lanes the scales of 128 columns came from shared
 // memory and the sums went out by single words: gate/up of 4096 tokens 281 us, down 243.)
 namespace pg {
-constexpr int kThreads = 384;                    // warps: 0 weights, 1 MMAs, 2 - 3 rows (2: tensor memory), 4 - 11 scale and add
-constexpr int kRegAux = 56, kRegAdd = 224;
-constexpr int kRegLaunch = 168;
-static_assert(128 * kRegAux + 256 * kRegAdd <= kThreads * kRegLaunch, "the shares must not exceed the launch's registers");
+constexpr int kThreads = 512;                    // warps: 0 weights, 1 MMAs, 2 - 7 rows (2: tensor memory), 8 - 15 scale and add
+constexpr int kRowWarps = 6;
+constexpr int kRegAux = 56, kRegAdd = 200;
+constexpr int kRegLaunch = 128;
+static_assert(256 * kRegAux + 256 * kRegAdd <= kThreads * kRegLaunch, "the shares must not exceed the launch's registers");
 constexpr uint32_t kStage = 3 * 16384, kStages = 4, kPut = kStages * kStage, kSmem = kPut + 8 * 2048 + 1024;   // 2 KB a warp on the way to coalesced stores
 }  // namespace pg
 
@@ -695,7 +696,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
     const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * pg::kStages, bar_set = bar_empty + 8 * pg::kStages, bar_free = bar_set + 16;
     if (tid == 0) {
-        for (uint32_t i = 0; i < pg::kStages; ++i) { mbar_init(bar_full + 8 * i, 1 + 2); mbar_init(bar_empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < pg::kStages; ++i) { mbar_init(bar_full + 8 * i, 1 + pg::kRowWarps); mbar_init(bar_empty + 8 * i, 1); }
         for (uint32_t i = 0; i < 2; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, 8); }
         mbar_fence_init();
     }
@@ -722,11 +723,11 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     // entry of the list of pairs for a row of a unit, the last one past its end (nobody looks at those rows)
     auto entry = [&](const GroupUnit& g, uint32_t row) -> uint32_t { const uint32_t p = g.p0 + min(row, g.n - 1); return kGrouped ? a.pairs[p] : p; };
 
-    if (warp >= 4) {
+    if (warp >= 8) {
         // ---- scale and add: TMEM lanes 32 q ..; of gate/up 64 columns of either matrix, else 128 columns of one tile
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(pg::kRegAdd));
-        const uint32_t q = warp & 3u, h = (warp - 4) >> 2, row = 32 * q + lane;
-        const uint32_t put = base + pg::kPut + (warp - 4) * 2048u;
+        const uint32_t q = warp & 3u, h = (warp - 8) >> 2, row = 32 * q + lane;
+        const uint32_t put = base + pg::kPut + (warp - 8) * 2048u;
         const uint32_t c0 = kGateUp ? 64 * h : 128 * h, c1 = kGateUp ? 128 + 64 * h : 128 * h + 64;   // first columns of the two runs of 64
         const uint32_t t0 = tmem + ((32 * q) << 16);
         uint32_t blk = 0, next = 0;                          // next: this row's entry of the list, read a unit ahead
@@ -810,8 +811,10 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(pg::kRegAux));
         if (warp >= 2) {
-            // ---- rows: four x 128 columns an instruction, every other four this warp's; a stage is announced two stages later, so that three are under way
+            // ---- rows: four x 128 columns an instruction.  A warp issues one about every 130 cycles, so six warps share a stage (two: 1.5 times the
+            // time of the whole at 128 pairs an expert); a stage is announced two stages later, so that three are under way.
             const uint32_t w = warp - 2, rr = lane >> 3, ck = lane & 7u;
+            constexpr int kFours = (32 + pg::kRowWarps - 1) / pg::kRowWarps;   // this warp's fours of rows: w, w + 6, ..
             uint32_t blk = 0;
             auto announce = [&](uint32_t i) {
                 umma::fence_smem_to_async();
@@ -819,25 +822,20 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                 if (lane == 0) mbar_arrive(bar_full + 8 * (i % pg::kStages));
             };
             GroupUnit g{};
-            uint32_t pr[2];                                  // entries of the warp's rows number lane and lane + 32, read a unit ahead; number i is row 8 (i / 4) + 4 w + i % 4
+            uint32_t next = 0;                               // entry of the warp's row number lane, read a unit ahead
             auto entries = [&](uint32_t u) {
                 g = s_list.at(u, live_i);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) pr[i] = entry(g, (lane + 32 * i) / 4 * 8 + 4 * w + (lane & 3u));
+                next = entry(g, ((lane >> 2) * pg::kRowWarps + w) * 4 + (lane & 3u));
             };
             if (u_first < u_end) entries(u_first);
             bool out = false;
             for (uint32_t u = u_first; u < u_end && !out; ++u) {
                 const uint32_t n = g.n;
-                uint32_t mine[2];                            // their rows of xq
+                const Fp8Place me = fp8_place<MODE>(a, next);
+                const uint8_t* src[kFours];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const Fp8Place r = fp8_place<MODE>(a, pr[i]);
-                    mine[i] = r.row == kFp8NoRow ? 0u : r.row;
-                }
-                uint32_t rows[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) rows[i] = __shfl_sync(0xFFFFFFFFu, mine[i >> 3], (4 * i + rr) & 31u);
+                for (int i = 0; i < kFours; ++i)
+                    src[i] = a.xq + (uint64_t)__shfl_sync(0xFFFFFFFFu, me.row == kFp8NoRow ? 0u : me.row, 4 * i + rr) * a.K + ck * 16u;
                 if (u + 1 < u_end) entries(u + 1);
                 for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
                     const uint32_t s = blk % pg::kStages;
@@ -845,12 +843,13 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                     if (blk >= pg::kStages) wait_bar(bar_empty + 8 * s, (blk / pg::kStages - 1) & 1u);
                     if (__any_sync(0xFFFFFFFFu, waits.out)) { out = true; break; }
                     const uint32_t dst = base + s * pg::kStage;
-                    const uint8_t* src = a.xq + kb * 128u + ck * 16u;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (8u * i < n)
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + umma::sw128_chunk(8 * i + 4 * w + rr, ck)), "l"(there ? src + (uint64_t)rows[i] * a.K : a.xq),
+                    for (int i = 0; i < kFours; ++i) {
+                        const uint32_t row0 = (i * pg::kRowWarps + w) * 4;
+                        if (row0 < n)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + umma::sw128_chunk(row0 + rr, ck)), "l"(there ? src[i] + kb * 128u : a.xq),
                                          "r"(there ? 16u : 0u) : "memory");
+                    }
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     if (blk >= 2) {
                         asm volatile("cp.async.wait_group 2;" ::: "memory");
