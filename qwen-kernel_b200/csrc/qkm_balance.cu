@@ -29,9 +29,11 @@ struct BalanceAcc {
 // V values a lane: column of value i
 template <bool VEC> __device__ __forceinline__ uint32_t bal_col(uint32_t lane, int i) { return VEC ? ((i >> 2) * 32 + lane) * 4 + (i & 3) : i * 32 + lane; }
 
-// a row's logits -> exp(logit - largest), 0 past the end; returns 1 / their sum; fine: bit i is set where value i's logit is finite
+// rows that a warp has under way at once
+template <int V> constexpr int bal_rows() { return V <= 8 ? 4 : 2; }
+
 template <int V, bool VEC>
-__device__ __forceinline__ float row_exp(const float* __restrict__ row, uint32_t E, uint32_t lane, float (&v)[V], uint32_t& fine) {
+__device__ __forceinline__ void row_load(const float* row, uint32_t E, uint32_t lane, float (&v)[V]) {
     if (VEC) {
 #pragma unroll
         for (int j = 0; j < V / 4; ++j) {
@@ -44,6 +46,15 @@ __device__ __forceinline__ float row_exp(const float* __restrict__ row, uint32_t
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = bal_col<VEC>(lane, i) < E ? row[bal_col<VEC>(lane, i)] : 0.f;
     }
+}
+__device__ __forceinline__ float warp_max(float v) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(r) : "f"(v));
+    return r;
+}
+// a row's logits -> exp(logit - largest), 0 past the end; returns 1 / their sum; fine: bit i is set where value i's logit is finite
+template <int V, bool VEC>
+__device__ __forceinline__ float row_exp(uint32_t E, uint32_t lane, float (&v)[V], uint32_t& fine) {
     float most = -INFINITY;
     fine = 0;
 #pragma unroll
@@ -52,8 +63,7 @@ __device__ __forceinline__ float row_exp(const float* __restrict__ row, uint32_t
         else v[i] = kFloor;
         if (bal_col<VEC>(lane, i) < E) most = fmaxf(most, v[i]);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+    most = warp_max(most);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -79,18 +89,32 @@ balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel
     __syncthreads();
     float p[V] = {};
     uint32_t kept = 0;
-    for (uint32_t t = blockIdx.x * kBalWarps + warp; t < n_tokens; t += gridDim.x * kBalWarps) {
-        if (mask && mask[t] == 0) continue;
-        float v[V];
-        uint32_t fine;
-        const float inv = row_exp<V, VEC>(logits + (size_t)t * E, E, lane, v, fine);
+    constexpr int R = bal_rows<V>();
+    const uint32_t step = gridDim.x * kBalWarps;
+    for (uint32_t t0 = blockIdx.x * kBalWarps + warp; t0 < n_tokens; t0 += R * step) {
+        float v[R][V];
+        uint32_t id[R];
+        bool in[R];
 #pragma unroll
-        for (int i = 0; i < V; ++i) p[i] += v[i] * inv;
-        if (lane < n_used) {
-            const uint32_t id = sel[t].ids[lane];
-            if (id < E) atomicAdd(&s_cnt[id], 1u);
+        for (int r = 0; r < R; ++r) {
+            const uint32_t t = t0 + r * step;      // (below 2^24 + 2^14)
+            in[r] = t < n_tokens && !(mask && mask[t] == 0);
+            id[r] = 0xFFFFFFFFu;
+            if (in[r]) {
+                row_load<V, VEC>(logits + (size_t)t * E, E, lane, v[r]);
+                if (lane < n_used) id[r] = sel[t].ids[lane];
+            }
         }
-        ++kept;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (in[r]) {                           // (the same for the whole warp)
+                uint32_t fine;
+                const float inv = row_exp<V, VEC>(E, lane, v[r], fine);
+#pragma unroll
+                for (int i = 0; i < V; ++i) p[i] += v[r][i] * inv;
+                if (id[r] < E) atomicAdd(&s_cnt[id[r]], 1u);
+                ++kept;
+            }
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) s_p[warp][bal_col<VEC>(lane, i)] = p[i];
@@ -143,31 +167,45 @@ balance_grad_kernel(const float* logits, const uint8_t* __restrict__ mask, const
     float g[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) g[i] = bal_col<VEC>(lane, i) < E ? (float)(unit * counts[bal_col<VEC>(lane, i)]) : 0.f;
-    for (uint32_t t = blockIdx.x * kBalWarps + warp; t < n_tokens; t += gridDim.x * kBalWarps) {
-        float v[V];
-        if (mask && mask[t] == 0) {
+    constexpr int R = bal_rows<V>();
+    const uint32_t step = gridDim.x * kBalWarps;
+    for (uint32_t t0 = blockIdx.x * kBalWarps + warp; t0 < n_tokens; t0 += R * step) {
+        float v[R][V];
+        bool in[R];
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = 0.f;
-        } else {
-            uint32_t fine;
-            const float inv = row_exp<V, VEC>(logits + (size_t)t * E, E, lane, v, fine);
-            float dot = 0.f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) { v[i] *= inv; dot += v[i] * g[i]; }
-            dot = warp_sum(dot);
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = fine >> i & 1u ? v[i] * (g[i] - dot) : 0.f;
+        for (int r = 0; r < R; ++r) {
+            const uint32_t t = t0 + r * step;
+            in[r] = t < n_tokens && !(mask && mask[t] == 0);
+            if (in[r]) row_load<V, VEC>(logits + (size_t)t * E, E, lane, v[r]);
         }
-        float* out = d_logits + (size_t)t * E;
-        if (VEC) {
 #pragma unroll
-            for (int j = 0; j < V / 4; ++j)
-                if (bal_col<VEC>(lane, 4 * j) < E)
-                    *reinterpret_cast<float4*>(out + bal_col<VEC>(lane, 4 * j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        } else {
+        for (int r = 0; r < R; ++r) {
+            const uint32_t t = t0 + r * step;
+            if (t >= n_tokens) break;
+            if (in[r]) {
+                uint32_t fine;
+                const float inv = row_exp<V, VEC>(E, lane, v[r], fine);
+                float dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (bal_col<VEC>(lane, i) < E) out[bal_col<VEC>(lane, i)] = v[i];
+                for (int i = 0; i < V; ++i) { v[r][i] *= inv; dot += v[r][i] * g[i]; }
+                dot = warp_sum(dot);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[r][i] = fine >> i & 1u ? v[r][i] * (g[i] - dot) : 0.f;
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[r][i] = 0.f;
+            }
+            float* out = d_logits + (size_t)t * E;
+            if (VEC) {
+#pragma unroll
+                for (int j = 0; j < V / 4; ++j)
+                    if (bal_col<VEC>(lane, 4 * j) < E)
+                        *reinterpret_cast<float4*>(out + bal_col<VEC>(lane, 4 * j)) = make_float4(v[r][4 * j], v[r][4 * j + 1], v[r][4 * j + 2], v[r][4 * j + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (bal_col<VEC>(lane, i) < E) out[bal_col<VEC>(lane, i)] = v[r][i];
+            }
         }
     }
 }
@@ -191,7 +229,7 @@ size_t balance_scratch_bytes() { return sizeof(BalanceAcc); }
 cudaError_t launch_balance(const Launch& L, const qkm_dims& d, const float* logits, const qkm_sel* sel, const uint8_t* mask, uint32_t n_tokens, float coef, void* scratch,
                            uint32_t* counts, float* probs, float* loss, uint32_t n_sms) {
     const cudaError_t e = bal_variant(d.n_expert, d.n_expert % 4 == 0 && ((uintptr_t)logits & 15u) == 0, [&](auto v, auto vec) {
-        return launch_kernel(Launch{L.stream, nullptr, true}, balance_kernel<v.value, vec.value>, dim3(bal_grid(n_tokens, n_sms, 2)), dim3(kBalThreads), 0, logits, sel, mask,
+        return launch_kernel(Launch{L.stream, nullptr, true}, balance_kernel<v.value, vec.value>, dim3(bal_grid(n_tokens, n_sms, 3)), dim3(kBalThreads), 0, logits, sel, mask,
                              n_tokens, d.n_expert, d.n_used, coef, (BalanceAcc*)scratch, counts, probs, loss);
     });
     L.count();

@@ -387,14 +387,19 @@ struct UnitList {
     // position in the list of the expert that unit u belongs to
     __device__ __forceinline__ uint32_t find(uint32_t u) const {
         uint32_t i = 0;
-        if (kGrouped && u < n_units)
+        if (kGrouped)
+#pragma unroll 1
             for (uint32_t step = kMax / 2; step; step >>= 1)
                 if (i + step < n_live && unit[i + step] <= u) i += step;
         return i;
     }
-    // unit u; i: its expert's position or an earlier one
+    __device__ __forceinline__ GroupUnit at(uint32_t u) const { return of(u, find(u)); }
+    // the same for units in ascending order: i is the position of the one before
     __device__ __forceinline__ GroupUnit at(uint32_t u, uint32_t& i) const {
         while (u >= unit[i + 1]) ++i;
+        return of(u, i);
+    }
+    __device__ __forceinline__ GroupUnit of(uint32_t u, uint32_t i) const {
         const uint32_t run = p1[i] - p0[i], parts = (run + PART - 1) / PART, k = u - unit[i], ru = k / parts, part = k - ru * parts;
         GroupUnit g;
         g.e = kGrouped ? expert[i] : 0u;
@@ -709,8 +714,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = s_tmem, n_units = s_list.n_units;
-    const uint32_t u_first = (uint32_t)((uint64_t)n_units * blockIdx.x / gridDim.x), u_end = (uint32_t)((uint64_t)n_units * (blockIdx.x + 1) / gridDim.x);
-    uint32_t live_i = s_list.find(u_first);
+    const uint32_t u_first = blockIdx.x, u_step = gridDim.x, u_end = n_units;   // (the row units of an expert at the same time in neighbouring blocks: 186 -> 177 us at 4096 tokens)
     Waits waits;
     auto wait_bar = [&](uint32_t b, uint32_t parity) {
         waits.wait([&] {
@@ -733,8 +737,8 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
         uint32_t blk = 0, next = 0;                          // next: this row's entry of the list, read a unit ahead
         bool ready = false;
         GroupUnit g{};
-        if (u_first < u_end) { g = s_list.at(u_first, live_i); next = entry(g, row); }
-        for (uint32_t u = u_first; u < u_end; ++u) {
+        if (u_first < u_end) { g = s_list.at(u_first); next = entry(g, row); }
+        for (uint32_t u = u_first; u < u_end; u += u_step) {
             const GroupUnit cur = g;
             const uint32_t mine = next;
             const Fp8Place me = fp8_place<MODE>(a, mine);
@@ -743,7 +747,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
             const float* ws1 = kGateUp ? a.w_scale[1] + ((uint64_t)cur.e * MB + cur.m0 / 128u) * KB : ws0;
             float x0 = xs[0], wa0 = ws0[0], wb0 = ws1[0];
             const float wt = me.row == kFp8NoRow ? 0.f : fp8_weight<MODE>(a, mine);
-            if (u + 1 < u_end) { g = s_list.at(u + 1, live_i); next = entry(g, row); }
+            if (u + u_step < u_end) { g = s_list.at(u + u_step); next = entry(g, row); }
             float acc[2][64];
 #pragma unroll
             for (int i = 0; i < 128; ++i) acc[i >> 6][i & 63] = 0.f;
@@ -824,19 +828,19 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
             GroupUnit g{};
             uint32_t next = 0;                               // entry of the warp's row number lane, read a unit ahead
             auto entries = [&](uint32_t u) {
-                g = s_list.at(u, live_i);
+                g = s_list.at(u);
                 next = entry(g, ((lane >> 2) * pg::kRowWarps + w) * 4 + (lane & 3u));
             };
             if (u_first < u_end) entries(u_first);
             bool out = false;
-            for (uint32_t u = u_first; u < u_end && !out; ++u) {
+            for (uint32_t u = u_first; u < u_end && !out; u += u_step) {
                 const uint32_t n = g.n;
                 const Fp8Place me = fp8_place<MODE>(a, next);
                 const uint8_t* src[kFours];
 #pragma unroll
                 for (int i = 0; i < kFours; ++i)
                     src[i] = a.xq + (uint64_t)__shfl_sync(0xFFFFFFFFu, me.row == kFp8NoRow ? 0u : me.row, 4 * i + rr) * a.K + ck * 16u;
-                if (u + 1 < u_end) entries(u + 1);
+                if (u + u_step < u_end) entries(u + u_step);
                 for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
                     const uint32_t s = blk % pg::kStages;
                     const bool there = kb * 128u + ck * 16u < a.K;
@@ -864,8 +868,8 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
             // ---- weights
             uint32_t blk = 0;
             bool out = false;
-            for (uint32_t u = u_first; u < u_end && !out; ++u) {
-                const GroupUnit g = s_list.at(u, live_i);
+            for (uint32_t u = u_first; u < u_end && !out; u += u_step) {
+                const GroupUnit g = s_list.at(u);
                 const uint32_t r0 = g.e * a.M + g.m0, r1 = kGateUp ? r0 : r0 + 128;
                 for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
                     const uint32_t s = blk % pg::kStages, dst = base + s * pg::kStage + 16384u, full = bar_full + 8 * s;
@@ -883,7 +887,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
         } else {
             // ---- MMAs
             const bool leader = umma::elect_one();
-            const uint32_t idesc = instr_desc_e4m3(128, 256), steps = (u_end - u_first) * KB;
+            const uint32_t idesc = instr_desc_e4m3(128, 256), steps = u_first < u_end ? ((u_end - u_first + u_step - 1) / u_step) * KB : 0u;
             const uint64_t da0 = umma::smem_desc(base);
             uint32_t s = 0, full_parity = 0, set = 0, free_parity = 1;
             uint64_t da = da0;
