@@ -6,6 +6,9 @@
 // N: tokens that the mask leaves.  The counts have no gradient.  A logit that is not finite is taken as -3.4e38, as the selection takes it
 // (shaders/moe_select.comp:28-34), and gets none.  A warp holds a row in registers, the same columns in the same lane for every row, so a lane adds up its
 // columns' probabilities - and keeps its columns' g - in registers.
+//
+// What bounds it at 32768 x 256: the loss (14.9 us; 33.5 MB, 5.1 at the copy rate) waits for the sums over blocks, about 5 us of it, and issues some
+// 25 instructions an element; the gradient (14.7 us; 67 MB, 10.2) is near its traffic.
 #include <type_traits>
 
 #include "qkm_common.cuh"
@@ -29,8 +32,10 @@ struct BalanceAcc {
 // V values a lane: column of value i
 template <bool VEC> __device__ __forceinline__ uint32_t bal_col(uint32_t lane, int i) { return VEC ? ((i >> 2) * 32 + lane) * 4 + (i & 3) : i * 32 + lane; }
 
-// rows that a warp has under way at once
-template <int V> constexpr int bal_rows() { return V <= 8 ? 4 : 2; }
+// rows that a warp has under way at once (32768 x 256: two 14.9 + 14.7 us, four 15.9 + 17.7; 32768 x 128: 13.0 + 12.8 against 11.9 + 11.5)
+template <int V> constexpr int bal_rows() { return V <= 4 ? 4 : 2; }
+
+constexpr float kLowest = -3.402823466e38f;   // stands for a logit past the end of a row, below any that counts
 
 template <int V, bool VEC>
 __device__ __forceinline__ void row_load(const float* row, uint32_t E, uint32_t lane, float (&v)[V]) {
@@ -38,13 +43,13 @@ __device__ __forceinline__ void row_load(const float* row, uint32_t E, uint32_t 
 #pragma unroll
         for (int j = 0; j < V / 4; ++j) {
             const uint32_t c = bal_col<VEC>(lane, 4 * j);
-            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+            float4 f = make_float4(kLowest, kLowest, kLowest, kLowest);
             if (c < E) f = *reinterpret_cast<const float4*>(row + c);
             v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = bal_col<VEC>(lane, i) < E ? row[bal_col<VEC>(lane, i)] : 0.f;
+        for (int i = 0; i < V; ++i) v[i] = bal_col<VEC>(lane, i) < E ? row[bal_col<VEC>(lane, i)] : kLowest;
     }
 }
 __device__ __forceinline__ float warp_max(float v) {
@@ -52,25 +57,36 @@ __device__ __forceinline__ float warp_max(float v) {
     asm("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(r) : "f"(v));
     return r;
 }
-// a row's logits -> exp(logit - largest), 0 past the end; returns 1 / their sum; fine: bit i is set where value i's logit is finite
+// e^x for x <= 0, to about 3 * 2^-24 of it, 0 below 2^-126: 2^t for t = x log2(e) rounded, times 1 + ln 2 times what the rounding of the product
+// (r, which an FMA gives exactly) and of log2(e) left out.
+__device__ __forceinline__ float exp_down(float x) {
+    constexpr float kLog2e = 1.44269504f, kRest = 1.92596303e-8f, kLn2 = 0.693147181f;   // log2(e) = kLog2e + kRest
+    x = fmaxf(x, -1e4f);                       // (0 from -88 on, and t stays finite)
+    const float t = x * kLog2e, r = fmaf(x, kLog2e, -t), c = fmaf(x, kRest * kLn2, r * kLn2);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    return fmaf(e, c, e);
+}
+// A row's logits -> exp(logit - largest), 0 past the end; returns 1 / their sum.  Where the largest is above the floor, what is at the floor, or past
+// the end, gives 0 by itself; `low` says that it is not, and the caller looks at every element then.
 template <int V, bool VEC>
-__device__ __forceinline__ float row_exp(uint32_t E, uint32_t lane, float (&v)[V], uint32_t& fine) {
-    float most = -INFINITY;
-    fine = 0;
+__device__ __forceinline__ float row_exp(uint32_t E, uint32_t lane, float (&v)[V], bool& low) {
+    float most = kLowest;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        if (isfinite(v[i])) fine |= 1u << i;
-        else v[i] = kFloor;
-        if (bal_col<VEC>(lane, i) < E) most = fmaxf(most, v[i]);
+        if (!(fabsf(v[i]) <= -kLowest)) v[i] = kFloor;
+        most = fmaxf(most, v[i]);
     }
     most = warp_max(most);
+    low = most <= kFloor;
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        v[i] = bal_col<VEC>(lane, i) < E ? expf(v[i] - most) : 0.f;
+        v[i] = exp_down(v[i] - most);
+        if (low && bal_col<VEC>(lane, i) >= E) v[i] = 0.f;
         sum += v[i];
     }
-    return 1.f / warp_sum(sum);
+    return __fdividef(1.f, warp_sum(sum));     // (1 <= sum <= 512)
 }
 
 template <int V, bool VEC>
@@ -108,8 +124,8 @@ balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel
 #pragma unroll
         for (int r = 0; r < R; ++r)
             if (in[r]) {                           // (the same for the whole warp)
-                uint32_t fine;
-                const float inv = row_exp<V, VEC>(E, lane, v[r], fine);
+                bool low;
+                const float inv = row_exp<V, VEC>(E, lane, v[r], low);
 #pragma unroll
                 for (int i = 0; i < V; ++i) p[i] += v[r][i] * inv;
                 if (id[r] < E) atomicAdd(&s_cnt[id[r]], 1u);
@@ -155,6 +171,13 @@ balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel
     }
 }
 
+template <int V>
+__device__ __forceinline__ void drop(float (&v)[V], int at) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i == at) v[i] = 0.f;
+}
+
 template <int V, bool VEC>
 __global__ void __launch_bounds__(kBalThreads)
 balance_grad_kernel(const float* logits, const uint8_t* __restrict__ mask, const uint32_t* __restrict__ counts, uint32_t n_tokens, uint32_t E, uint32_t n_used, float coef,
@@ -183,14 +206,18 @@ balance_grad_kernel(const float* logits, const uint8_t* __restrict__ mask, const
             const uint32_t t = t0 + r * step;
             if (t >= n_tokens) break;
             if (in[r]) {
-                uint32_t fine;
-                const float inv = row_exp<V, VEC>(E, lane, v[r], fine);
+                bool low;
+                const float inv = row_exp<V, VEC>(E, lane, v[r], low);
                 float dot = 0.f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) { v[r][i] *= inv; dot += v[r][i] * g[i]; }
                 dot = warp_sum(dot);
 #pragma unroll
-                for (int i = 0; i < V; ++i) v[r][i] = fine >> i & 1u ? v[r][i] * (g[i] - dot) : 0.f;
+                for (int i = 0; i < V; ++i) v[r][i] *= g[i] - dot;
+                if (low)                           // logits at the floor count here: those that are not finite get no gradient
+#pragma unroll 1
+                    for (int i = 0; i < V; ++i)
+                        if (bal_col<VEC>(lane, i) < E && !isfinite(logits[(size_t)t * E + bal_col<VEC>(lane, i)])) drop(v[r], i);
             } else {
 #pragma unroll
                 for (int i = 0; i < V; ++i) v[r][i] = 0.f;
@@ -217,9 +244,12 @@ cudaError_t bal_variant(uint32_t E, bool vec, F f) {
     if (E <= 256) return vec ? f(std::integral_constant<int, 8>{}, std::true_type{}) : f(std::integral_constant<int, 8>{}, std::false_type{});
     return vec ? f(std::integral_constant<int, 16>{}, std::true_type{}) : f(std::integral_constant<int, 16>{}, std::false_type{});
 }
-uint32_t bal_grid(uint32_t n_tokens, uint32_t n_sms, uint32_t per_sm) {
-    const uint32_t want = (n_tokens + kBalWarps - 1) / kBalWarps;
-    return want < 1 ? 1u : want < n_sms * per_sm ? want : n_sms * per_sm;
+// Blocks: as many as the SMs hold, or fewer where that gives every warp the same number of rounds.
+uint32_t bal_grid(uint32_t n_tokens, uint32_t n_sms, uint32_t per_sm, uint32_t rows) {
+    const uint32_t most = n_sms * per_sm, want = (n_tokens + kBalWarps - 1) / kBalWarps;
+    if (want <= most) return want < 1 ? 1u : want;
+    const uint32_t round = most * kBalWarps * rows, rounds = (n_tokens + round - 1) / round;
+    return (n_tokens + rounds * rows * kBalWarps - 1) / (rounds * rows * kBalWarps);
 }
 
 }  // namespace
@@ -229,7 +259,7 @@ size_t balance_scratch_bytes() { return sizeof(BalanceAcc); }
 cudaError_t launch_balance(const Launch& L, const qkm_dims& d, const float* logits, const qkm_sel* sel, const uint8_t* mask, uint32_t n_tokens, float coef, void* scratch,
                            uint32_t* counts, float* probs, float* loss, uint32_t n_sms) {
     const cudaError_t e = bal_variant(d.n_expert, d.n_expert % 4 == 0 && ((uintptr_t)logits & 15u) == 0, [&](auto v, auto vec) {
-        return launch_kernel(Launch{L.stream, nullptr, true}, balance_kernel<v.value, vec.value>, dim3(bal_grid(n_tokens, n_sms, 3)), dim3(kBalThreads), 0, logits, sel, mask,
+        return launch_kernel(Launch{L.stream, nullptr, true}, balance_kernel<v.value, vec.value>, dim3(bal_grid(n_tokens, n_sms, v.value <= 8 ? 4 : 3, bal_rows<v.value>())), dim3(kBalThreads), 0, logits, sel, mask,
                              n_tokens, d.n_expert, d.n_used, coef, (BalanceAcc*)scratch, counts, probs, loss);
     });
     L.count();
@@ -241,7 +271,7 @@ cudaError_t launch_balance_grad(const Launch& L, const qkm_dims& d, const float*
     if (n_tokens == 0) return cudaSuccess;
     const bool vec = d.n_expert % 4 == 0 && (((uintptr_t)logits | (uintptr_t)d_logits) & 15u) == 0;
     const cudaError_t e = bal_variant(d.n_expert, vec, [&](auto v, auto ve) {
-        return launch_kernel(Launch{L.stream, nullptr, true}, balance_grad_kernel<v.value, ve.value>, dim3(bal_grid(n_tokens, n_sms, 4)), dim3(kBalThreads), 0, logits, mask,
+        return launch_kernel(Launch{L.stream, nullptr, true}, balance_grad_kernel<v.value, ve.value>, dim3(bal_grid(n_tokens, n_sms, v.value == 8 ? 6 : 4, bal_rows<v.value>())), dim3(kBalThreads), 0, logits, mask,
                              counts, n_tokens, d.n_expert, d.n_used, coef, d_loss, d_logits);
     });
     L.count();
