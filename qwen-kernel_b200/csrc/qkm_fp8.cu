@@ -93,7 +93,7 @@ namespace {
 constexpr int kRowsThreads = 256, kRowsWarps = kRowsThreads / 32;
 
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -102,8 +102,8 @@ __device__ __forceinline__ uint4 ld16(const uint8_t* p, bool there) { return the
 
 template <int MODE> constexpr int rows_mats() { return MODE == kFp8GateUp || MODE == kFp8SharedGateUp ? 2 : 1; }
 
-// 16 weight rows from m0 of expert e times rows [p0, p0 + 8 NT) of its run; NT: groups of eight rows
-template <int MODE, int NT>
+// U: column blocks that a warp loads ahead of their MMAs.  16 weight rows from m0 of expert e times rows [p0, p0 + 8 NT) of its run; NT: groups of eight rows
+template <int MODE, int NT, int U>
 __device__ __forceinline__ void rows_tile(const Fp8Args& a, uint32_t e, uint32_t m0, uint32_t p0, uint32_t p1, float* s_red) {
     constexpr int MATS = rows_mats<MODE>();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
@@ -132,37 +132,47 @@ __device__ __forceinline__ void rows_tile(const Fp8Args& a, uint32_t e, uint32_t
     }
     const bool has0 = m0 + g < a.M, has1 = m0 + g + 8 < a.M;
     float acc[MATS][NT][4] = {};
-    for (uint32_t kb = warp; kb < KB; kb += kRowsWarps) {
-        const uint32_t c0 = kb * 128 + t * 16;
-        const bool in[2] = {c0 < a.K, c0 + 64 < a.K};
-        uint4 wv[MATS][2][2];
+    for (uint32_t kb0 = warp; kb0 < KB; kb0 += U * kRowsWarps) {
+        uint4 wv[U][MATS][2][2], xv[U][NT][2];
+        float ws[U][MATS], x0[U][NT], x1[U][NT];
 #pragma unroll
-        for (int m = 0; m < MATS; ++m)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                wv[m][c][0] = ld16(wrow[m] + c0 + 64 * c, has0 && in[c]);
-                wv[m][c][1] = ld16(wrow[m] + (uint64_t)8 * a.K + c0 + 64 * c, has1 && in[c]);
-            }
-        float ws[MATS];
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) ws[m] = __ldg(wsc[m] + kb);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            uint4 xv[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) xv[c] = ld16(xrow[j] + c0 + 64 * c, xrow[j] != nullptr && in[c]);
-            const float x0 = xsc[j][0] ? xsc[j][0][kb] : 0.f, x1 = xsc[j][1] ? xsc[j][1][kb] : 0.f;
+        for (int u = 0; u < U; ++u) {
+            const uint32_t kb = kb0 + u * kRowsWarps, c0 = kb * 128 + t * 16;
+            const bool there = kb < KB, in[2] = {there && c0 < a.K, there && c0 + 64 < a.K};
 #pragma unroll
             for (int m = 0; m < MATS; ++m) {
-                float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    mma_e4m3(d, wv[m][c][0].x, wv[m][c][1].x, wv[m][c][0].y, wv[m][c][1].y, xv[c].x, xv[c].y);
-                    mma_e4m3(d, wv[m][c][0].z, wv[m][c][1].z, wv[m][c][0].w, wv[m][c][1].w, xv[c].z, xv[c].w);
+                    wv[u][m][c][0] = ld16(wrow[m] + c0 + 64 * c, has0 && in[c]);
+                    wv[u][m][c][1] = ld16(wrow[m] + (uint64_t)8 * a.K + c0 + 64 * c, has1 && in[c]);
                 }
-                const float s0 = x0 * ws[m], s1 = x1 * ws[m];
-                acc[m][j][0] += d[0] * s0; acc[m][j][1] += d[1] * s1; acc[m][j][2] += d[2] * s0; acc[m][j][3] += d[3] * s1;
+                ws[u][m] = there ? __ldg(wsc[m] + kb) : 0.f;
             }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) xv[u][j][c] = ld16(xrow[j] + c0 + 64 * c, xrow[j] != nullptr && in[c]);
+                x0[u][j] = there && xsc[j][0] ? xsc[j][0][kb] : 0.f;
+                x1[u][j] = there && xsc[j][1] ? xsc[j][1][kb] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (kb0 + u * kRowsWarps >= KB) break;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const uint4 &w0 = wv[u][m][c][0], &w1 = wv[u][m][c][1], &x = xv[u][j][c];
+                        mma_e4m3(d, w0.x, w1.x, w0.y, w1.y, x.x, x.y);
+                        mma_e4m3(d, w0.z, w1.z, w0.w, w1.w, x.z, x.w);
+                    }
+                    const float s0 = x0[u][j] * ws[u][m], s1 = x1[u][j] * ws[u][m];
+                    acc[m][j][0] += d[0] * s0; acc[m][j][1] += d[1] * s1; acc[m][j][2] += d[2] * s0; acc[m][j][3] += d[3] * s1;
+                }
         }
     }
     // s_red[warp][mat][column][16 rows]
@@ -213,7 +223,7 @@ __device__ __forceinline__ uint32_t live_experts(const Fp8Args& a, uint16_t* s_l
     return total;
 }
 
-template <int MODE, int NT>
+template <int MODE, int NT, int U>
 __global__ void __launch_bounds__(kRowsThreads)
 fp8_rows_kernel(const Fp8Args a) {
     constexpr uint32_t kCols = 8 * NT;
@@ -228,7 +238,7 @@ fp8_rows_kernel(const Fp8Args a) {
         const uint32_t i = (uint32_t)(u / tiles), m0 = (uint32_t)(u - (uint64_t)i * tiles) * 16u;
         uint32_t e = 0, p0 = 0, p1 = a.n;
         if (kGrouped) { e = s_live[i]; fp8_run(a, e, p0, p1); }
-        for (uint32_t p = p0 + blockIdx.y * kCols; p < p1; p += gridDim.y * kCols) rows_tile<MODE, NT>(a, e, m0, p, p1, s_red);
+        for (uint32_t p = p0 + blockIdx.y * kCols; p < p1; p += gridDim.y * kCols) rows_tile<MODE, NT, U>(a, e, m0, p, p1, s_red);
     }
 }
 
@@ -244,8 +254,12 @@ cudaError_t rows_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
         const uint32_t gx = (uint32_t)(kGrouped ? (most < n_sms * 8ull ? most : n_sms * 8ull) : (most < 0x7FFFFFFF ? most : 0x7FFFFFFF));
         return launch_kernel(P, kernel, dim3(gx, chunks < 65535 ? chunks : 65535), dim3(kRowsThreads), 0, a);
     };
-    if (kGrouped ? a.n <= 8 : a.n <= 8) e = go(fp8_rows_kernel<MODE, 1>, 8);
-    else e = go(fp8_rows_kernel<MODE, 2>, 16);
+    // As many blocks of columns at once as a warp has (one row, K = 4096, M = 2048: two 6.4 us, four 3.9, 16 rows 7.3 and 5.4; K = 2048, where it has two, four cost occupancy: M = 8192
+    // 6.2 against 9.7)
+    const bool wide = a.K > 2048;
+    if (rows_mats<MODE>() == 2) e = a.n <= 8 ? go(fp8_rows_kernel<MODE, 1, 1>, 8) : go(fp8_rows_kernel<MODE, 2, 1>, 16);
+    else if (a.n <= 8) e = wide ? go(fp8_rows_kernel<MODE, 1, 4>, 8) : go(fp8_rows_kernel<MODE, 1, 2>, 8);
+    else e = wide ? go(fp8_rows_kernel<MODE, 2, 4>, 16) : go(fp8_rows_kernel<MODE, 2, 2>, 16);
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();
 }

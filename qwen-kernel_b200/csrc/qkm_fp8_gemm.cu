@@ -6,6 +6,8 @@
 // row and a run of columns inside one block of 128 weight rows, so the scale is one number a thread and the scaling one FMA an element.
 #include <cuda.h>
 
+#include <cmath>
+
 #include "qkm_common.cuh"
 #include "qkm_fp8.cuh"
 #include "qkm_umma.cuh"
@@ -20,13 +22,16 @@ constexpr int kAux = 4, kAdders = 8;
 constexpr int kRegAux = 40, kRegAdd = 232;       // registers a thread after the split
 constexpr int kRegLaunch = 168;
 static_assert(kAux * 32 * kRegAux + kAdders * 32 * kRegAdd <= kThreads * kRegLaunch, "the shares must not exceed the launch's registers");
-constexpr uint32_t kBN = 256;                    // weight rows of a tile; CG blocks share a tile of CG * 128 rows
-template <int CG> struct Tile {
-    static constexpr uint32_t kRowsW = kBN / CG;                      // weight rows that a block loads
+// BN weight rows a tile; CG blocks share a tile of CG * 128 rows
+template <int CG, int BN> struct Tile {
+    static constexpr uint32_t kRowsW = BN / CG;                       // weight rows that a block loads
     static constexpr uint32_t kStage = 128 * 128 + kRowsW * 128;
-    static constexpr uint32_t kStages = CG == 2 ? 6 : 4;
+    static constexpr uint32_t kStages = 196608u / kStage < 8 ? 196608u / kStage : 8;
+    static constexpr uint32_t kSets = BN == 256 ? 2 : 4;              // tensor-memory column sets
     static constexpr uint32_t kPut = kStages * kStage;                // 4 KB a warp: the way of the results to coalesced stores
     static constexpr uint32_t kSmem = kPut + kAdders * 4096 + 1024;   // (+ what aligning the start may take)
+    static constexpr int kCols = BN / 2;                              // columns of a thread
+    static constexpr int kLoad = kCols < 64 ? kCols : 64;             // and of a load
 };
 }  // namespace tg
 
@@ -127,12 +132,34 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
+// 64, 32 or 16 columns of this warp's lanes, waited for
+__device__ __forceinline__ void tmem_load(uint32_t t, float (&v)[64]) {
+    float (&lo)[32] = reinterpret_cast<float (&)[32]>(v[0]), (&hi)[32] = reinterpret_cast<float (&)[32]>(v[32]);
+    tmem_ld32(t, lo);
+    tmem_ld32(t + 32, hi);
+    tmem_ld_done(lo);
+    tmem_ld_done(hi);
+}
+__device__ __forceinline__ void tmem_load(uint32_t t, float (&v)[32]) {
+    tmem_ld32(t, v);
+    tmem_ld_done(v);
+}
+__device__ __forceinline__ void tmem_load(uint32_t t, float (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+                   "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+                 : "r"(t));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(v[i]));
+}
 // acc += v * s, two elements an instruction
-__device__ __forceinline__ void add_scaled(float (&acc)[64], int at, const float (&v)[32], float s) {
+template <int N>
+__device__ __forceinline__ void add_scaled(float* acc, const float (&v)[N], float s) {
     uint64_t s2;
     asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
 #pragma unroll
-    for (int i = 0; i < 32; i += 2)
+    for (int i = 0; i < N; i += 2)
         asm("{\n"
             ".reg .b64 v, c;\n"
             "mov.b64 v, {%2, %3};\n"
@@ -140,7 +167,7 @@ __device__ __forceinline__ void add_scaled(float (&acc)[64], int at, const float
             "fma.rn.f32x2 c, v, %4, c;\n"
             "mov.b64 {%0, %1}, c;\n"
             "}\n"
-            : "+f"(acc[at + i]), "+f"(acc[at + i + 1]) : "f"(v[i]), "f"(v[i + 1]), "l"(s2));
+            : "+f"(acc[i]), "+f"(acc[i + 1]) : "f"(v[i]), "f"(v[i + 1]), "l"(s2));
 }
 
 struct WideArgs {
@@ -152,20 +179,20 @@ struct WideArgs {
     uint32_t* status;
 };
 
-template <int CG>
+template <int CG, int BN>
 __global__ void __launch_bounds__(tg::kThreads, 1)
 fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap w_map) {
-    using T = tg::Tile<CG>;
+    using T = tg::Tile<CG, BN>;
     extern __shared__ uint8_t smem_dyn[];
-    __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 4];
+    __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets];
     __shared__ uint32_t s_tmem;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t rank = CG == 2 ? cluster_rank() : 0u, unit0 = blockIdx.x / CG, units = gridDim.x / CG;
     const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
-    const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * T::kStages, bar_set = bar_empty + 8 * T::kStages, bar_free = bar_set + 16;
+    const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * T::kStages, bar_set = bar_empty + 8 * T::kStages, bar_free = bar_set + 8 * T::kSets;
     if (tid == 0) {
         for (uint32_t i = 0; i < T::kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
-        for (uint32_t i = 0; i < 2; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, CG * tg::kAdders); }
+        for (uint32_t i = 0; i < T::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, CG * tg::kAdders); }
         mbar_fence_init();
     }
     if (warp == 2) tmem_take<CG>(smem_addr(&s_tmem));
@@ -189,71 +216,73 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
     };
 
     if (warp >= (uint32_t)tg::kAux) {
-        // ---- scale and add: TMEM lanes 32 q .., columns 128 h .. of a set, weight rows of one block of 128
+        // ---- scale and add: TMEM lanes 32 q .., half h of a set's columns, weight rows of one block of 128
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(tg::kRegAdd));
         const uint32_t q = warp & 3u, h = (warp - tg::kAux) >> 2;
         const uint32_t put = base + T::kPut + (warp - tg::kAux) * 4096u;
-        const uint32_t t0 = tmem + ((32 * q) << 16) + h * 128u, free0 = CG == 2 ? in_first(bar_free) : bar_free;
-        uint32_t blk = 0;                                                // column blocks so far: set blk % 2
+        const uint32_t t0 = tmem + ((32 * q) << 16) + h * T::kCols, free0 = CG == 2 ? in_first(bar_free) : bar_free;
+        uint32_t set = 0, parity = 0;                                    // the next set, and its barrier's phase
         bool ready = false;                                              // the next set's barrier is through
         for (uint32_t u = unit0; u < a.n_tiles; u += units) {
             const uint32_t xt = u % a.x_tiles, wt = u / a.x_tiles;
-            const uint32_t r0 = (xt * CG + rank) * 128u + 32 * q, m0 = wt * tg::kBN + h * 128u;
+            const uint32_t r0 = (xt * CG + rank) * 128u + 32 * q, m0 = wt * BN + h * T::kCols;
             const float* xs = a.x_scale + (size_t)min(r0 + lane, a.n - 1) * a.KB;
             const float* ws = a.w_scale + (size_t)min(m0 / 128u, a.MB - 1) * a.KB;
-            float acc[2][64];
+            constexpr int kParts = T::kCols / T::kLoad;
+            float acc[kParts][T::kLoad];
 #pragma unroll
-            for (int i = 0; i < 128; ++i) acc[i >> 6][i & 63] = 0.f;
+            for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                for (int i = 0; i < T::kLoad; ++i) acc[p][i] = 0.f;
             float x0 = xs[0], w0 = ws[0];                                // (the next block's scales are on their way while this one's are used)
-            for (uint32_t kb = 0; kb < a.KB; ++kb, ++blk) {
-                const uint32_t set = blk & 1u, t = t0 + set * 256u;
+            for (uint32_t kb = 0; kb < a.KB; ++kb) {
+                const uint32_t t = t0 + set * BN;
                 const float xc = x0, wc = w0;
                 if (kb + 1 < a.KB) { x0 = xs[kb + 1]; w0 = ws[kb + 1]; }
-                if (!ready) wait_bar(bar_set + 8 * set, (blk >> 1) & 1u);
+                if (!ready) wait_bar(bar_set + 8 * set, parity);
                 umma::fence_after_sync();
                 const float s = xc * wc;
-                float v[2][32];
-                tmem_ld32(t, v[0]);
-                tmem_ld32(t + 32, v[1]);
-                tmem_ld_done(v[0]);
-                tmem_ld_done(v[1]);
-                add_scaled(acc[0], 0, v[0], s);
-                add_scaled(acc[0], 32, v[1], s);
-                tmem_ld32(t + 64, v[0]);
-                tmem_ld32(t + 96, v[1]);
-                tmem_ld_done(v[0]);
-                tmem_ld_done(v[1]);
-                umma::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) { if (CG == 2) mbar_arrive_cluster(free0 + 8 * set); else mbar_arrive(free0 + 8 * set); }
-                ready = mbar_test(bar_set + 8 * (set ^ 1u), ((blk + 1) >> 1) & 1u);   // its answer comes while the additions run
-                add_scaled(acc[1], 0, v[0], s);
-                add_scaled(acc[1], 32, v[1], s);
+#pragma unroll
+                for (int p = 0; p < kParts; ++p) {
+                    float v[T::kLoad];
+                    tmem_load(t + T::kLoad * p, v);
+                    if (p + 1 == kParts) {
+                        umma::fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) { if (CG == 2) mbar_arrive_cluster(free0 + 8 * set); else mbar_arrive(free0 + 8 * set); }
+                        if (++set == T::kSets) { set = 0; parity ^= 1u; }
+                        ready = mbar_test(bar_set + 8 * set, parity);    // its answer comes while the additions run
+                    }
+                    add_scaled(acc[p], v, s);
+                }
             }
             if (__any_sync(0xFFFFFFFFu, waits.out)) break;
-            // 32 rows x 32 columns at a time through shared memory: lanes along the columns for the stores
+            // 32 rows x 32 columns at a time (16, where a thread has no more) through shared memory: lanes along the columns for the stores
+            constexpr int kPiece = T::kCols < 32 ? T::kCols : 32, kQuads = kPiece / 4, kRows = 32 / kQuads;   // rows of a store
+            auto place = [](uint32_t r, uint32_t j) -> uint32_t { return r * (4u * kPiece) + ((j ^ (kQuads == 8 ? r & 7u : (r >> 1) & (kQuads - 1))) << 4); };
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < T::kCols / kPiece; ++c) {
                 __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(put + lane * 128u + ((j ^ (lane & 7u)) << 4)), "f"(acc[c >> 1][32 * (c & 1) + 4 * j]),
-                                 "f"(acc[c >> 1][32 * (c & 1) + 4 * j + 1]), "f"(acc[c >> 1][32 * (c & 1) + 4 * j + 2]), "f"(acc[c >> 1][32 * (c & 1) + 4 * j + 3]) : "memory");
+                for (int j = 0; j < kQuads; ++j) {
+                    const float* e = &acc[c * kPiece / T::kLoad][c * kPiece % T::kLoad + 4 * j];
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(put + place(lane, j)), "f"(e[0]), "f"(e[1]), "f"(e[2]), "f"(e[3]) : "memory");
+                }
                 __syncwarp();
-                const uint32_t j = lane & 7u, m = m0 + 32 * c + 4 * j;
+                const uint32_t j = lane % kQuads, m = m0 + kPiece * c + 4 * j;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t r = 4 * i + (lane >> 3), row = r0 + r;
-                    const uint4 o = lds128(put + r * 128u + ((j ^ (r & 7u)) << 4));
+                for (int i = 0; i < 32 / kRows; ++i) {
+                    const uint32_t r = kRows * i + lane / kQuads, row = r0 + r;
+                    const uint4 o = lds128(put + place(r, j));
                     if (row >= a.n) continue;
                     float* y = a.y + (size_t)row * a.M + m;
                     if (a.vec) {
                         if (m < a.M) *reinterpret_cast<uint4*>(y) = o;
                     } else {
-                        const uint32_t e[4] = {o.x, o.y, o.z, o.w};
+                        const uint32_t w[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
-                            if (m + k < a.M) y[k] = __uint_as_float(e[k]);
+                            if (m + k < a.M) y[k] = __uint_as_float(w[k]);
                     }
                 }
             }
@@ -275,7 +304,7 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
                         const uint32_t full = CG == 2 ? in_first(bar_full + 8 * s) : bar_full + 8 * s;
                         if (rank == 0) mbar_expect_tx(bar_full + 8 * s, CG * T::kStage);
                         tma_tile<CG>(dst, &x_map, kb * 128u, (xt * CG + rank) * 128u, full);
-                        tma_tile<CG>(dst + 16384u, &w_map, kb * 128u, wt * tg::kBN + rank * T::kRowsW, full);
+                        tma_tile<CG>(dst + 16384u, &w_map, kb * 128u, wt * BN + rank * T::kRowsW, full);
                     }
                     __syncwarp();
                 }
@@ -286,7 +315,7 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
             // ---- MMAs.  The way from a set's return to the next MMA into it is part of the loop that bounds the kernel: as few
             // instructions as may be, counters that are added to instead of remainders.
             const bool leader = umma::elect_one();
-            const uint32_t idesc = instr_desc_e4m3(128 * CG, tg::kBN);
+            const uint32_t idesc = instr_desc_e4m3(128 * CG, BN);
             const uint32_t steps = unit0 < a.n_tiles ? ((a.n_tiles - unit0 + units - 1) / units) * a.KB : 0u;
             const uint64_t da0 = umma::smem_desc(base);
             uint32_t s = 0, full_parity = 0, set = 0, free_parity = 1;   // (the first pass over the sets waits for the phase before the first)
@@ -297,15 +326,14 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
                 umma::fence_after_sync();
                 if (leader) {   // (after a wait that ran out the MMAs run on: their operands are in bounds, and the tile is never stored)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_e4m3_ss<CG>(tmem + set * 256u, da + 2 * j, da + 1024 + 2 * j, idesc, j != 0);
+                    for (int j = 0; j < 4; ++j) mma_e4m3_ss<CG>(tmem + set * BN, da + 2 * j, da + 1024 + 2 * j, idesc, j != 0);
                     commit_all<CG>(bar_set + 8 * set);
                     commit_all<CG>(bar_empty + 8 * s);
                 }
                 __syncwarp();
                 da += T::kStage / 16;
                 if (++s == T::kStages) { s = 0; da = da0; full_parity ^= 1u; }
-                set ^= 1u;
-                free_parity ^= set ^ 1u;
+                if (++set == T::kSets) { set = 0; free_parity ^= 1u; }
             }
         }
     }
@@ -414,7 +442,7 @@ __device__ __forceinline__ void tmem_ld8f(uint32_t taddr, float (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_load(uint32_t t, float (&v)[8]) { tmem_ld8f(t, v); }
+__device__ __forceinline__ void tmem_ld(uint32_t t, float (&v)[8]) { tmem_ld8f(t, v); }
 // waits for the loads, whose registers are used behind it
 template <int N> __device__ __forceinline__ void tmem_done(float (&a)[N], float (&b)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -507,8 +535,8 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                     const uint32_t col = (2 * j + h) * T::kChunk;
                     if (col >= g.n) continue;
                     float v0[T::kChunk], v1[T::kChunk];
-                    tmem_load(t + col, v0);
-                    tmem_load(t + NT + col, v1);
+                    tmem_ld(t + col, v0);
+                    tmem_ld(t + NT + col, v1);
                     tmem_done(v0, v1);
 #pragma unroll
                     for (int i = 0; i < T::kChunk; i += 4) {
@@ -765,7 +793,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                     for (int c = 0; c < 3; ++c) {
                         tmem_ld32(t + (c < 2 ? c0 + 32 * c : c1), v);
                         tmem_ld_done(v);
-                        add_scaled(acc[c >> 1], 32 * (c & 1), v, c < 2 ? s : xc * (kGateUp ? wbc : wac));
+                        add_scaled(&acc[c >> 1][32 * (c & 1)], v, c < 2 ? s : xc * (kGateUp ? wbc : wac));
                     }
                     tmem_ld32(t + c1 + 32, v);
                     tmem_ld_done(v);
@@ -774,7 +802,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_free + 8 * set);
                 ready = mbar_test(bar_set + 8 * (set ^ 1u), ((blk + 1) >> 1) & 1u);
-                if (work) add_scaled(acc[1], 32, v, xc * (kGateUp ? wbc : wac));
+                if (work) add_scaled(&acc[1][32], v, xc * (kGateUp ? wbc : wac));
             }
             if (__any_sync(0xFFFFFFFFu, waits.out)) break;
             if (!work) continue;
@@ -942,17 +970,17 @@ cudaError_t check_registers() {
     return regs >= Want ? cudaSuccess : cudaErrorInvalidKernelImage;
 }
 
-template <int CG>
+template <int CG, int BN>
 cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
-    using T = tg::Tile<CG>;
-    if (const cudaError_t e = allow_dynamic_smem<fp8_wide_kernel<CG>>((int)T::kSmem)) return e;
-    if (const cudaError_t e = check_registers<fp8_wide_kernel<CG>, tg::kRegLaunch>()) return e;
+    using T = tg::Tile<CG, BN>;
+    if (const cudaError_t e = allow_dynamic_smem<fp8_wide_kernel<CG, BN>>((int)T::kSmem)) return e;
+    if (const cudaError_t e = check_registers<fp8_wide_kernel<CG, BN>, tg::kRegLaunch>()) return e;
     CUtensorMap xm, wm;
     if (!fp8_map(&xm, a.xq, a.n, a.K, 128) || !fp8_map(&wm, a.w[0], a.M, a.K, T::kRowsW)) return cudaErrorInvalidValue;
     WideArgs w{};
     w.w_scale = a.w_scale[0]; w.x_scale = a.x_scale; w.y = a.out; w.M = a.M; w.n = a.n; w.KB = (a.K + 127) / 128; w.MB = (a.M + 127) / 128;
     w.x_tiles = (a.n + 128 * CG - 1) / (128 * CG);
-    const uint64_t tiles = (uint64_t)w.x_tiles * ((a.M + tg::kBN - 1) / tg::kBN);
+    const uint64_t tiles = (uint64_t)w.x_tiles * ((a.M + BN - 1) / BN);
     if (tiles > 0x7FFFFFFFu) return cudaErrorInvalidValue;
     w.n_tiles = (uint32_t)tiles;
     w.vec = a.M % 4 == 0 && ((uintptr_t)a.out & 15u) == 0;
@@ -966,7 +994,7 @@ cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = CG; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = CG == 2 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_wide_kernel<CG>, w, xm, wm);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, fp8_wide_kernel<CG, BN>, w, xm, wm);
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -1012,19 +1040,45 @@ cudaError_t group_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     return mean > 24 ? pairs_launch<MODE>(L, a, n_sms) : group_launch<MODE, 32>(L, a, n_sms);
 }
 
+// Which kernel a dense product takes: the least of these estimates, in us, fitted to measurements from 1 to 4096 rows, 1000 to 151,936 weight rows and K = 1040 to 4096.
+// Tiles go over the machine in waves whose length is that of a tile (at K = 2048: 5.0 us for 128 x 32, 5.5 for 128 x 64, 8.5 for 128 x 256; of pairs of blocks 6.2 for
+// 256 x 128, 8.5 for 256 x 256), so that few rows or a small matrix want small tiles and large ones those that read least.  Of at most 32 rows the weights are what is
+// read: by warps straight from memory where the matrix is small (16 x 4096 x 2048 5.2 us, group tiles 9.8, 128 x 32 8.4), through the group kernel's ring where it is large
+// (1 x 151,936 x 2048 55 us against 60 and 65; 16 rows 57 against 111 and 59).
+cudaError_t dense_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
+    const double mb = (double)a.M * a.K * 1e-6, k = a.K / 2048.0;
+    auto waves = [&](uint32_t rows, uint32_t cols, uint32_t slots) {
+        const uint64_t tiles = (uint64_t)((a.n + rows - 1) / rows) * ((a.M + cols - 1) / cols);
+        return (double)((tiles + slots - 1) / slots) * k;
+    };
+    const double rows = (a.n <= 8 ? 0.19 : 0.3 * ((a.n + 15) / 16)) * mb - 0.5;
+    const double group = a.n > 32 ? 1e30 : fmax(6.3 * waves(32, 256, n_sms), mb / 5.9), read = mb / 4.9;
+    const double wide[5] = {5.0 * waves(128, 32, n_sms), 5.5 * waves(128, 64, n_sms), 6.2 * waves(256, 128, n_sms / 2), 8.5 * waves(128, 256, n_sms), 8.5 * waves(256, 256, n_sms / 2)};
+    int best = 0;
+    for (int i = 1; i < 5; ++i)
+        if (wide[i] <= wide[best]) best = i;
+    const double tiles = fmax(wide[best], read);
+    if (rows <= group && rows <= tiles) return launch_fp8_rows(L, kFp8Dense, a, n_sms);
+    if (group <= tiles) return group_launch<kFp8Dense, 32>(L, a, n_sms);
+    switch (best) {
+        case 0: return wide_launch<1, 32>(L, a, n_sms);
+        case 1: return wide_launch<1, 64>(L, a, n_sms);
+        case 2: return wide_launch<2, 128>(L, a, n_sms);
+        case 3: return wide_launch<1, 256>(L, a, n_sms);
+        default: return wide_launch<2, 256>(L, a, n_sms);
+    }
+}
+
 }  // namespace
 
 cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) {
     if (a.n == 0 || a.M == 0) return cudaSuccess;
     if (a.K >= 128) switch (mode) {
-        case kFp8Dense:
-            if (a.n > 256) return wide_launch<2>(L, a, n_sms);
-            if (a.n > 16) return group_any<kFp8Dense>(L, a, n_sms);
-            break;
+        case kFp8Dense: return dense_any(L, a, n_sms);
         case kFp8GateUp: return group_any<kFp8GateUp>(L, a, n_sms);
         case kFp8Down: return group_any<kFp8Down>(L, a, n_sms);
-        case kFp8SharedGateUp: if (a.n > 16) return group_any<kFp8SharedGateUp>(L, a, n_sms); break;
-        case kFp8SharedDown: if (a.n > 16) return group_any<kFp8SharedDown>(L, a, n_sms); break;
+        case kFp8SharedGateUp: if (a.n > 64) return pairs_launch<kFp8SharedGateUp>(L, a, n_sms); break;
+        case kFp8SharedDown: if (a.n > 64) return pairs_launch<kFp8SharedDown>(L, a, n_sms); break;
     }
     return launch_fp8_rows(L, mode, a, n_sms);
 }
