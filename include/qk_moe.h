@@ -290,7 +290,7 @@ QKM_API int qkm_fp8_gemm(qkm_ctx *c, const void *W, const float *w_scale, const 
 /* The experts' products, as qkm_moe_gateup_grouped, qkm_moe_down_grouped, qkm_moe_shared_gateup and qkm_moe_shared_down with
  * the context's n_embd, n_ff, n_expert and n_used.  xq: the tokens' rows [n_tokens][n_embd]; hq: rows [n_tokens][n_used + 1][n_ff], e.g.
  * qkm_fp8_quantize of h with n = n_tokens * (n_used + 1).  gate/up writes the slots that the list names (the shared form slot n_used),
- * f32; down multiplies by the record's routing weight (w_shared).  Pairs that name a token or a slot that there is none of are skipped. */
+ * f32; down multiplies by the record's routing weight (w_shared).  h, contrib and y2 start on 16-byte boundaries; n_tokens < 2^27 (rows of qkm_fp8_gemm: 2^28).  Pairs that name a token or a slot that there is none of are skipped. */
 QKM_API int qkm_moe_gateup_grouped_fp8(qkm_ctx *c, const void *gate_exps, const float *gate_scale,
                                        const void *up_exps, const float *up_scale, const void *xq,
                                        const float *x_scale, const uint32_t *offsets,

@@ -1133,7 +1133,9 @@ int fp8_product(qkm_ctx* c, const char* name, int mode, const void* w0, const fl
                 const uint32_t* pairs, const qkm_sel* sel, float* out, uint32_t M, uint32_t K, uint32_t n) {
     if (K == 0 || K % 16) return fail(c, QKM_ERR_ARG, "%s: K=%u must be a multiple of 16", name, K);
     if (!aligned16(w0) || !aligned16(w1) || !aligned16(xq)) return fail(c, QKM_ERR_ARG, "%s: E4M3 rows must start on 16 bytes", name);
-    if (n >= 1u << 28) return fail(c, QKM_ERR_BOUNDS, "%s: %u rows exceed 2^28", name, n);
+    if (mode != kFp8Dense && !aligned16(out)) return fail(c, QKM_ERR_ARG, "%s: the results must start on 16 bytes", name);
+    // (rows of hq and of the results, n * (n_used + 1) at most, are counted in 32 bits)
+    if (n >= (mode == kFp8Dense ? 1u << 28 : 1u << 27)) return fail(c, QKM_ERR_BOUNDS, "%s: %u rows exceed 2^%d", name, n, mode == kFp8Dense ? 28 : 27);
     OnDevice on(c->device);
     Fp8Args a{};
     a.w[0] = (const uint8_t*)w0; a.w[1] = (const uint8_t*)w1; a.w_scale[0] = s0; a.w_scale[1] = s1;

@@ -24,7 +24,6 @@ struct Fp8Args {
     float* out;
     uint32_t M, K, n;              // n: rows (dense), tokens otherwise
     uint32_t n_experts, n_used;
-    uint32_t vec;                  // out may be stored 16 bytes at a time
     uint32_t* status;
 };
 

@@ -370,30 +370,27 @@ template <int NT> struct Tile {
 
 struct GroupUnit { uint32_t e, m0, p0, n; };     // expert, first weight row, first pair, pairs
 
-// The units of a product: experts that have pairs (of a dense product or the shared expert the one matrix), their runs of pairs cut into parts of PART,
+// The units of a product: experts that have pairs (of a dense product or the shared expert the one matrix), their runs of pairs cut into parts of PART at most,
 // every part with all row units of the expert; the parts of a row unit next to one another.
-template <int MODE, int PART>
+// SORTED: parts of one expert of the same length, experts in descending order of it, units handed out to and fro, so that every block gets as much as the others (with units
+// of 4 to 128 pairs dealt in the experts' order the busiest SM had 1.4 times the average).
+template <int MODE, int PART, uint32_t ROWS, bool SORTED>
 struct UnitList {
-    static constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    static constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
     static constexpr uint32_t kMax = kGrouped ? gg::kMaxExperts : 1u;
     uint32_t unit[kMax + 1], p0[kMax], p1[kMax];     // per live expert: first unit, run
     uint32_t scan[16][2], n_live, n_units;
     uint16_t expert[kMax];
+    uint32_t size[SORTED && kGrouped ? kMax / 4 : 1];   // a byte an expert: length of its parts
 
-    // by all threads of the block (256 or more; two experts each); __syncthreads behind it
-    __device__ __forceinline__ void make(const Fp8Args& a) {
-        const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, row_units = kGateUp ? (a.M + 127) / 128 : (a.M + 255) / 256;
-        uint32_t q0[2] = {}, q1[2] = {}, units[2], c = 0, v = 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint32_t e = 2 * tid + i;
-            if (kGrouped) { if (e < a.n_experts) fp8_run(a, e, q0[i], q1[i]); }
-            else if (e == 0) q1[i] = a.n;
-            units[i] = (q1[i] - q0[i] + PART - 1) / PART * row_units;
-            c += units[i] ? 1u : 0u;
-            v += units[i];
-        }
-        const uint32_t c_mine = c, v_mine = v;
+    static __device__ __forceinline__ uint32_t part_size(uint32_t run) {
+        if (!SORTED || run <= (uint32_t)PART) return SORTED ? run : (uint32_t)PART;
+        const uint32_t parts = (run + PART - 1) / PART;
+        return ((run + parts - 1) / parts + 3u) & ~3u;
+    }
+    // inclusive sums over the block's threads of two numbers
+    __device__ __forceinline__ void sums(uint32_t& c, uint32_t& v) {
+        const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t c1 = __shfl_up_sync(0xFFFFFFFFu, c, o), v1 = __shfl_up_sync(0xFFFFFFFFu, v, o);
@@ -402,16 +399,75 @@ struct UnitList {
         if (lane == 31) { scan[warp][0] = c; scan[warp][1] = v; }
         __syncthreads();
         for (uint32_t w = 0; w < warp; ++w) { c += scan[w][0]; v += scan[w][1]; }
-        if (tid == blockDim.x - 1) { n_live = c; n_units = v; unit[c] = v; }
-        c -= c_mine; v -= v_mine;
+    }
+    // by all threads of the block (256 or more; two experts each); __syncthreads behind it
+    __device__ __forceinline__ void make(const Fp8Args& a) {
+        const uint32_t tid = threadIdx.x, row_units = (a.M + ROWS - 1) / ROWS;
+        uint32_t q0[2] = {}, q1[2] = {}, units[2], e[2] = {2 * tid, 2 * tid + 1}, c = 0, v = 0;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (units[i]) {
-                expert[c] = (uint16_t)(2 * tid + i); p0[c] = q0[i]; p1[c] = q1[i]; unit[c] = v;
+        for (int i = 0; i < 2; ++i) {
+            if (kGrouped) { if (e[i] < a.n_experts) fp8_run(a, e[i], q0[i], q1[i]); }
+            else if (e[i] == 0) q1[i] = a.n;
+        }
+        if constexpr (SORTED && kGrouped) {
+            uint8_t* s = reinterpret_cast<uint8_t*>(size);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (e[i] < kMax) s[e[i]] = (uint8_t)part_size(q1[i] - q0[i]);
+            __syncthreads();
+            // an expert's place: how many have longer parts, or as long ones and a lower number
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (q1[i] <= q0[i]) continue;
+                const uint32_t mine = s[e[i]] * 0x01010101u;
+                uint32_t at = 0;
+                for (uint32_t w = 0; w < (a.n_experts + 3) / 4; ++w) {
+                    const uint32_t longer = __vcmpgtu4(size[w], mine), same = __vcmpeq4(size[w], mine);
+                    const uint32_t before = w < e[i] / 4 ? 0xFFFFFFFFu : w > e[i] / 4 ? 0u : (1u << (8 * (e[i] & 3u))) - 1u;
+                    at += __popc(longer | (same & before));
+                }
+                at >>= 3;
+                expert[at] = (uint16_t)e[i]; p0[at] = q0[i]; p1[at] = q1[i];
                 ++c;
+            }
+            c = __syncthreads_count(c > 0) + __syncthreads_count(c > 1);   // live experts
+            if (tid == 0) n_live = c;
+            const uint32_t live = c;
+            c = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                units[i] = e[i] < live ? (p1[e[i]] - p0[e[i]] + PART - 1) / PART * row_units : 0u;
                 v += units[i];
             }
+            const uint32_t mine = v;
+            sums(c, v);
+            if (tid == blockDim.x - 1) { n_units = v; unit[live] = v; }
+            v -= mine;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (e[i] < live) { unit[e[i]] = v; v += units[i]; }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                units[i] = (q1[i] - q0[i] + PART - 1) / PART * row_units;
+                c += units[i] ? 1u : 0u;
+                v += units[i];
+            }
+            const uint32_t c_mine = c, v_mine = v;
+            sums(c, v);
+            if (tid == blockDim.x - 1) { n_live = c; n_units = v; unit[c] = v; }
+            c -= c_mine; v -= v_mine;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (units[i]) {
+                    expert[c] = (uint16_t)e[i]; p0[c] = q0[i]; p1[c] = q1[i]; unit[c] = v;
+                    ++c;
+                    v += units[i];
+                }
+        }
     }
+    // number of this block's r-th unit, dealt to and fro; n_units or more: none
+    __device__ __forceinline__ uint32_t number(uint32_t r) const { return r * gridDim.x + (r & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
     // position in the list of the expert that unit u belongs to
     __device__ __forceinline__ uint32_t find(uint32_t u) const {
         uint32_t i = 0;
@@ -428,12 +484,12 @@ struct UnitList {
         return of(u, i);
     }
     __device__ __forceinline__ GroupUnit of(uint32_t u, uint32_t i) const {
-        const uint32_t run = p1[i] - p0[i], parts = (run + PART - 1) / PART, k = u - unit[i], ru = k / parts, part = k - ru * parts;
+        const uint32_t run = p1[i] - p0[i], len = part_size(run), parts = (run + len - 1) / len, k = u - unit[i], ru = k / parts, part = k - ru * parts;
         GroupUnit g;
         g.e = kGrouped ? expert[i] : 0u;
-        g.m0 = ru * (kGateUp ? 128u : 256u);
-        g.p0 = p0[i] + part * PART;
-        g.n = min((uint32_t)PART, run - part * PART);
+        g.m0 = ru * ROWS;
+        g.p0 = p0[i] + part * len;
+        g.n = min(len, run - part * len);
         return g;
     }
 };
@@ -475,7 +531,7 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     extern __shared__ uint8_t smem_dyn[];
     __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets + 2 * gg::kScales + gg::kMeta];
     __shared__ uint32_t s_tmem;
-    __shared__ UnitList<MODE, NT> s_list;
+    __shared__ UnitList<MODE, NT, kGateUp ? 128u : 256u, false> s_list;
     __shared__ uint64_t s_out[gg::kMeta][NT];        // per unit: where a column's results go, ~0: nowhere; its routing weight
     __shared__ float s_wt[gg::kMeta][NT];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -704,6 +760,35 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
 }
 
+// Where a warp's 32 rows of results go: of the rows 8 i + lane / 4 the row of `out`, kFp8NoRow nowhere.
+struct OutRows { uint32_t row[4]; };
+__device__ __forceinline__ OutRows out_rows(uint32_t mine) {
+    OutRows o;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) o.row[i] = __shfl_sync(0xFFFFFFFFu, mine, 8 * i + ((threadIdx.x & 31u) >> 2));
+    return o;
+}
+// 16 columns of them, by way of 2 KB of shared memory at `put`: four lanes a row for the stores.  All loads ahead of the stores and no branch but their predicates: with
+// the address, a shuffle and a branch ahead of each the stores took 350 cycles apiece, 60 us of down at 4096 tokens.
+__device__ __forceinline__ void put_columns(const float (&r)[16], uint32_t put, const OutRows& rows, float* out, uint32_t M) {
+    const uint32_t lane = threadIdx.x & 31u, j = lane & 3u;
+    __syncwarp();
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+        asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(put + lane * 64u + ((i ^ ((lane >> 1) & 3u)) << 4)), "f"(r[4 * i]), "f"(r[4 * i + 1]), "f"(r[4 * i + 2]), "f"(r[4 * i + 3])
+                     : "memory");
+    __syncwarp();
+    uint4 o[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t row = 8 * i + (lane >> 2);
+        o[i] = lds128(put + row * 64u + ((j ^ ((row >> 1) & 3u)) << 4));
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+        if (rows.row[i] != kFp8NoRow) *reinterpret_cast<uint4*>(out + (uint64_t)rows.row[i] * M + 4 * j) = o[i];
+}
+
 // ---- the same with the pairs as lanes, for experts of many pairs ------------------------------------------------------------------------
 // A unit is up to 128 pairs (the MMAs' rows, a lane each) times 256 weight rows: the gate and the up rows of a 128-row tile, or two tiles of one matrix.  What a
 // thread scales is then one row's, as in the dense kernel: an FMA for two elements and nothing else.  (With the weight rows as lanes the scales of 128 columns came from shared
@@ -711,7 +796,7 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
 namespace pg {
 constexpr int kThreads = 512;                    // warps: 0 weights, 1 MMAs, 2 - 7 rows (2: tensor memory), 8 - 15 scale and add
 constexpr int kRowWarps = 6;
-constexpr int kRegAux = 56, kRegAdd = 200;
+constexpr int kRegAux = 64, kRegAdd = 192;
 constexpr int kRegLaunch = 128;
 static_assert(256 * kRegAux + 256 * kRegAdd <= kThreads * kRegLaunch, "the shares must not exceed the launch's registers");
 constexpr uint32_t kStage = 3 * 16384, kStages = 4, kPut = kStages * kStage, kSmem = kPut + 8 * 2048 + 1024;   // 2 KB a warp on the way to coalesced stores
@@ -724,7 +809,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     extern __shared__ uint8_t smem_dyn[];
     __shared__ __align__(8) unsigned long long s_bar[2 * pg::kStages + 4];
     __shared__ uint32_t s_tmem;
-    __shared__ UnitList<MODE, 128> s_list;
+    __shared__ UnitList<MODE, 128, kGateUp ? 128u : 256u, true> s_list;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
     const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * pg::kStages, bar_set = bar_empty + 8 * pg::kStages, bar_free = bar_set + 16;
@@ -742,7 +827,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     __syncthreads();
     umma::fence_after_sync();
     const uint32_t tmem = s_tmem, n_units = s_list.n_units;
-    const uint32_t u_first = blockIdx.x, u_step = gridDim.x, u_end = n_units;   // (the row units of an expert at the same time in neighbouring blocks: 186 -> 177 us at 4096 tokens)
+    const uint32_t u_end = n_units;
     Waits waits;
     auto wait_bar = [&](uint32_t b, uint32_t parity) {
         waits.wait([&] {
@@ -765,8 +850,8 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
         uint32_t blk = 0, next = 0;                          // next: this row's entry of the list, read a unit ahead
         bool ready = false;
         GroupUnit g{};
-        if (u_first < u_end) { g = s_list.at(u_first); next = entry(g, row); }
-        for (uint32_t u = u_first; u < u_end; u += u_step) {
+        if (s_list.number(0) < u_end) { g = s_list.at(s_list.number(0)); next = entry(g, row); }
+        for (uint32_t r = 0, u; (u = s_list.number(r)) < u_end; ++r) {
             const GroupUnit cur = g;
             const uint32_t mine = next;
             const Fp8Place me = fp8_place<MODE>(a, mine);
@@ -775,7 +860,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
             const float* ws1 = kGateUp ? a.w_scale[1] + ((uint64_t)cur.e * MB + cur.m0 / 128u) * KB : ws0;
             float x0 = xs[0], wa0 = ws0[0], wb0 = ws1[0];
             const float wt = me.row == kFp8NoRow ? 0.f : fp8_weight<MODE>(a, mine);
-            if (u + u_step < u_end) { g = s_list.at(u + u_step); next = entry(g, row); }
+            if (const uint32_t u1 = s_list.number(r + 1); u1 < u_end) { g = s_list.at(u1); next = entry(g, row); }
             float acc[2][64];
 #pragma unroll
             for (int i = 0; i < 128; ++i) acc[i >> 6][i & 63] = 0.f;
@@ -806,38 +891,14 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
             }
             if (__any_sync(0xFFFFFFFFu, waits.out)) break;
             if (!work) continue;
-            // 32 rows x 16 columns at a time through shared memory, four lanes a row for the stores
-            const uint64_t out0 = row >= cur.n || me.row == kFp8NoRow ? ~0ull : me.out * a.M;
+            const OutRows to = out_rows(row >= cur.n || me.row == kFp8NoRow ? kFp8NoRow : (uint32_t)me.out);
             const uint32_t m0 = cur.m0 + (kGateUp ? 64 * h : 128 * h);
 #pragma unroll
             for (int c = 0; c < (kGateUp ? 4 : 8); ++c) {
                 float r[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    r[i] = kGateUp ? silu_times(acc[0][16 * c + i], acc[1][16 * c + i]) : MODE == kFp8Dense ? acc[c >> 2][16 * (c & 3) + i] : wt * acc[c >> 2][16 * (c & 3) + i];
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(put + lane * 64u + ((j ^ ((lane >> 1) & 3u)) << 4)), "f"(r[4 * j]), "f"(r[4 * j + 1]), "f"(r[4 * j + 2]),
-                                 "f"(r[4 * j + 3]) : "memory");
-                __syncwarp();
-                const uint32_t j = lane & 3u, m = m0 + 16 * c + 4 * j;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t rr = 8 * i + (lane >> 2);
-                    const uint4 o = lds128(put + rr * 64u + ((j ^ ((rr >> 1) & 3u)) << 4));
-                    const uint64_t at = __shfl_sync(0xFFFFFFFFu, out0, rr);
-                    if (at == ~0ull) continue;
-                    float* y = a.out + at + m;
-                    if (a.vec) {
-                        if (m < a.M) *reinterpret_cast<uint4*>(y) = o;
-                    } else {
-                        const uint32_t e[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (m + k < a.M) y[k] = __uint_as_float(e[k]);
-                    }
-                }
+                for (int i = 0; i < 16; ++i) r[i] = kGateUp ? silu_times(acc[0][(16 * c + i) & 63], acc[1][(16 * c + i) & 63]) : wt * acc[c >> 2][16 * (c & 3) + i];
+                put_columns(r, put, to, a.out + m0 + 16 * c, a.M);
             }
         }
     } else {
@@ -859,16 +920,16 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                 g = s_list.at(u);
                 next = entry(g, ((lane >> 2) * pg::kRowWarps + w) * 4 + (lane & 3u));
             };
-            if (u_first < u_end) entries(u_first);
+            if (s_list.number(0) < u_end) entries(s_list.number(0));
             bool out = false;
-            for (uint32_t u = u_first; u < u_end && !out; u += u_step) {
+            for (uint32_t r = 0, u; (u = s_list.number(r)) < u_end && !out; ++r) {
                 const uint32_t n = g.n;
                 const Fp8Place me = fp8_place<MODE>(a, next);
                 const uint8_t* src[kFours];
 #pragma unroll
                 for (int i = 0; i < kFours; ++i)
                     src[i] = a.xq + (uint64_t)__shfl_sync(0xFFFFFFFFu, me.row == kFp8NoRow ? 0u : me.row, 4 * i + rr) * a.K + ck * 16u;
-                if (u + u_step < u_end) entries(u + u_step);
+                if (const uint32_t u1 = s_list.number(r + 1); u1 < u_end) entries(u1);
                 for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
                     const uint32_t s = blk % pg::kStages;
                     const bool there = kb * 128u + ck * 16u < a.K;
@@ -896,7 +957,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
             // ---- weights
             uint32_t blk = 0;
             bool out = false;
-            for (uint32_t u = u_first; u < u_end && !out; u += u_step) {
+            for (uint32_t r = 0, u; (u = s_list.number(r)) < u_end && !out; ++r) {
                 const GroupUnit g = s_list.at(u);
                 const uint32_t r0 = g.e * a.M + g.m0, r1 = kGateUp ? r0 : r0 + 128;
                 for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
@@ -915,7 +976,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
         } else {
             // ---- MMAs
             const bool leader = umma::elect_one();
-            const uint32_t idesc = instr_desc_e4m3(128, 256), steps = u_first < u_end ? ((u_end - u_first + u_step - 1) / u_step) * KB : 0u;
+            const uint32_t idesc = instr_desc_e4m3(128, 256), rounds = u_end / gridDim.x, steps = (rounds + (s_list.number(rounds) < u_end ? 1u : 0u)) * KB;
             const uint64_t da0 = umma::smem_desc(base);
             uint32_t s = 0, full_parity = 0, set = 0, free_parity = 1;
             uint64_t da = da0;
@@ -935,6 +996,218 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                 set ^= 1u;
                 free_parity ^= set ^ 1u;
             }
+        }
+    }
+    umma::fence_before_sync();
+    const int any_timed_out = __syncthreads_or(waits.out ? 1 : 0);
+    if (any_timed_out) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies and MMAs still under way end long before this does
+    if (warp == 2) umma::tmem_dealloc(tmem, 512);
+    if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
+}
+
+// ---- down products of many pairs and short sums ------------------------------------------------------------------------------------------
+// Of four column blocks or fewer a unit's results take as long to store as its sums to make.  Here a unit is 128 pairs times 512 weight rows, in tiles of 128: the pairs' rows stay in
+// shared memory for all of them, tiles come through a ring, and the two halves of the warps that scale and add take the tiles in turns, so that one stores while the other
+// adds.  (down of 4096 tokens, K = 512: the kernel above 174 us, 70 of them stores that nothing overlaps.)
+namespace dg {
+constexpr uint32_t kMaxBlocks = 4, kRows = 512, kX = kMaxBlocks * 16384, kStages = 4, kSets = 4;
+constexpr uint32_t kW = 2 * kX, kPut = kW + kStages * 16384, kSmem = kPut + 8 * 2048 + 1024;   // x twice, weight tiles, 2 KB a warp on the way to coalesced stores
+}  // namespace dg
+
+template <int MODE>
+__global__ void __launch_bounds__(pg::kThreads, 1)
+fp8_down_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map) {
+    constexpr bool kGrouped = MODE == kFp8Down;
+    static_assert(MODE == kFp8Down || MODE == kFp8SharedDown, "one matrix");
+    extern __shared__ uint8_t smem_dyn[];
+    __shared__ __align__(8) unsigned long long s_bar[4 + 2 * dg::kStages + 3 * dg::kSets];
+    __shared__ uint32_t s_tmem;
+    __shared__ UnitList<MODE, 128, dg::kRows, true> s_list;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
+    const uint32_t bar_xfull = smem_addr(s_bar), bar_xempty = bar_xfull + 16, bar_full = bar_xempty + 16, bar_empty = bar_full + 8 * dg::kStages;
+    const uint32_t bar_set = bar_empty + 8 * dg::kStages, bar_free = bar_set + 16 * dg::kSets;   // sets: [half][set]
+    if (tid == 0) {
+        for (uint32_t i = 0; i < 2; ++i) { mbar_init(bar_xfull + 8 * i, pg::kRowWarps); mbar_init(bar_xempty + 8 * i, 1); }
+        for (uint32_t i = 0; i < dg::kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < dg::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_set + 8 * (dg::kSets + i), 1); mbar_init(bar_free + 8 * i, 4); }
+        mbar_fence_init();
+    }
+    if (warp == 2) { umma::tmem_alloc(smem_addr(&s_tmem), 512); umma::tmem_relinquish(); }
+    umma::fence_before_sync();
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t KB = fp8_blocks(a.K), MB = fp8_blocks(a.M);
+    s_list.make(a);
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = s_tmem, u_end = s_list.n_units;
+    Waits waits;
+    auto wait_bar = [&](uint32_t b, uint32_t parity) {
+        waits.wait([&] {
+#pragma unroll 1
+            for (int i = 0; i < 64; ++i)
+                if (mbar_try_wait(b, parity)) return true;
+            return mbar_wait_timed(b, parity);
+        });
+    };
+    auto entry = [&](const GroupUnit& g, uint32_t row) -> uint32_t { const uint32_t p = g.p0 + min(row, g.n - 1); return kGrouped ? a.pairs[p] : p; };
+    auto tiles_of = [&](const GroupUnit& g) -> uint32_t { return (min(dg::kRows, a.M - g.m0) + 127) / 128; };
+
+    if (warp >= 8) {
+        // ---- scale and add: TMEM lanes 32 q .., every other tile this half's
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(pg::kRegAdd));
+        const uint32_t q = warp & 3u, h = (warp - 8) >> 2, row = 32 * q + lane;
+        const uint32_t put = base + dg::kPut + (warp - 8) * 2048u, t0 = tmem + ((32 * q) << 16);
+        // A phase of a barrier is told from the next one only, and a set's next use may be the other half's: each half has barriers of its own.
+        const uint32_t set0 = bar_set + 8 * dg::kSets * h;
+        uint32_t tile = 0, phases = 0, next = 0;             // tiles before; a bit a set: parity of its next phase; this row's entry of the list, read a unit ahead
+        if (s_list.number(0) < u_end) next = entry(s_list.at(s_list.number(0)), row);
+        for (uint32_t r = 0, u; (u = s_list.number(r)) < u_end; ++r) {
+            const GroupUnit g = s_list.at(u);
+            const uint32_t tiles = tiles_of(g);
+            const Fp8Place me = fp8_place<MODE>(a, next);
+            const float wt = me.row == kFp8NoRow ? 0.f : fp8_weight<MODE>(a, next);
+            const OutRows to = out_rows(row >= g.n || me.row == kFp8NoRow ? kFp8NoRow : (uint32_t)me.out);
+            const bool work = 32 * q < g.n;                  // some row of this warp's is there
+            float x[dg::kMaxBlocks];
+#pragma unroll
+            for (uint32_t kb = 0; kb < dg::kMaxBlocks; ++kb) x[kb] = kb < KB ? a.x_scale[(uint64_t)(me.row == kFp8NoRow ? 0u : me.row) * KB + kb] : 0.f;
+            if (const uint32_t u1 = s_list.number(r + 1); u1 < u_end) next = entry(s_list.at(u1), row);
+            const float* ws = a.w_scale[0] + ((uint64_t)g.e * MB + g.m0 / 128u) * KB;
+            for (uint32_t i = 0; i < tiles; ++i, ++tile) {
+                if ((tile & 1u) != h) continue;
+                float w[dg::kMaxBlocks];
+#pragma unroll
+                for (uint32_t kb = 0; kb < dg::kMaxBlocks; ++kb) w[kb] = kb < KB ? ws[i * KB + kb] : 0.f;
+                float acc[2][64];
+#pragma unroll
+                for (int j = 0; j < 128; ++j) acc[j >> 6][j & 63] = 0.f;
+#pragma unroll
+                for (uint32_t kb = 0; kb < dg::kMaxBlocks; ++kb) {
+                    if (kb >= KB) break;
+                    const uint32_t set = (tile * KB + kb) % dg::kSets, t = t0 + set * 128u;
+                    wait_bar(set0 + 8 * set, phases >> set & 1u);
+                    phases ^= 1u << set;
+                    umma::fence_after_sync();
+                    const float s = x[kb] * w[kb];
+                    float v[32];
+                    if (work) {
+#pragma unroll
+                        for (int c = 0; c < 3; ++c) {
+                            tmem_ld32(t + 32 * c, v);
+                            tmem_ld_done(v);
+                            add_scaled(&acc[c >> 1][32 * (c & 1)], v, s);
+                        }
+                        tmem_ld32(t + 96, v);
+                        tmem_ld_done(v);
+                    }
+                    umma::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_free + 8 * set);
+                    if (work) add_scaled(&acc[1][32], v, s);
+                }
+                if (!work || __any_sync(0xFFFFFFFFu, waits.out)) continue;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    float r[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) r[j] = wt * acc[c >> 2][16 * (c & 3) + j];
+                    put_columns(r, put, to, a.out + g.m0 + i * 128u + 16 * c, a.M);
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(pg::kRegAux));
+        if (warp >= 2) {
+            // ---- rows: four x 128 columns an instruction, all of a unit's into one of two places
+            const uint32_t w = warp - 2, rr = lane >> 3, ck = lane & 7u;
+            constexpr int kFours = (32 + pg::kRowWarps - 1) / pg::kRowWarps;   // this warp's fours of rows: w, w + 6, ..
+            uint32_t unit = 0, n = 0, next = 0;              // next: entry of the warp's row number lane, read a unit ahead
+            auto entries = [&](uint32_t u) {
+                const GroupUnit g = s_list.at(u);
+                n = g.n;
+                next = entry(g, ((lane >> 2) * pg::kRowWarps + w) * 4 + (lane & 3u));
+            };
+            if (s_list.number(0) < u_end) entries(s_list.number(0));
+            for (uint32_t u; (u = s_list.number(unit)) < u_end; ++unit) {
+                const uint32_t rows = n, place = unit & 1u, dst = base + place * dg::kX;
+                const Fp8Place me = fp8_place<MODE>(a, next);
+                const uint8_t* src[kFours];
+#pragma unroll
+                for (int i = 0; i < kFours; ++i)
+                    src[i] = a.xq + (uint64_t)__shfl_sync(0xFFFFFFFFu, me.row == kFp8NoRow ? 0u : me.row, 4 * i + rr) * a.K + ck * 16u;
+                if (const uint32_t u1 = s_list.number(unit + 1); u1 < u_end) entries(u1);
+                if (unit >= 2) wait_bar(bar_xempty + 8 * place, (unit / 2 - 1) & 1u);
+                if (__any_sync(0xFFFFFFFFu, waits.out)) break;
+                for (uint32_t kb = 0; kb < KB; ++kb) {
+                    const bool there = kb * 128u + ck * 16u < a.K;
+#pragma unroll
+                    for (int i = 0; i < kFours; ++i) {
+                        const uint32_t row0 = (i * pg::kRowWarps + w) * 4;
+                        if (row0 < rows)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + kb * 16384u + umma::sw128_chunk(row0 + rr, ck)), "l"(there ? src[i] + kb * 128u : a.xq),
+                                         "r"(there ? 16u : 0u) : "memory");
+                    }
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                umma::fence_smem_to_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_xfull + 8 * place);
+            }
+        } else if (warp == 0) {
+            // ---- weight tiles
+            uint32_t blk = 0;
+            bool out = false;
+            for (uint32_t r = 0, u; (u = s_list.number(r)) < u_end && !out; ++r) {
+                const GroupUnit g = s_list.at(u);
+                const uint32_t steps = tiles_of(g) * KB;
+                uint32_t row = g.e * a.M + g.m0, kb = 0;
+                for (uint32_t i = 0; i < steps; ++i, ++blk) {
+                    const uint32_t s = blk % dg::kStages, full = bar_full + 8 * s;
+                    if (blk >= dg::kStages) wait_bar(bar_empty + 8 * s, (blk / dg::kStages - 1) & 1u);
+                    if (__any_sync(0xFFFFFFFFu, waits.out)) { out = true; break; }   // a barrier that still counts bytes takes no second arrival
+                    if (lane == 0) {
+                        mbar_expect_tx(full, 16384u);
+                        tma_tile<1>(base + dg::kW + s * 16384u, &map, kb * 128u, row, full);
+                    }
+                    __syncwarp();
+                    if (++kb == KB) { kb = 0; row += 128; }
+                }
+            }
+            for (uint32_t i = blk > dg::kStages ? blk - dg::kStages : 0; i < blk && !out; ++i) wait_bar(bar_empty + 8 * (i % dg::kStages), (i / dg::kStages) & 1u);
+        } else {
+            // ---- MMAs
+            const bool leader = umma::elect_one();
+            const uint32_t idesc = instr_desc_e4m3(128, 128);
+            const uint64_t dx0 = umma::smem_desc(base), dw0 = umma::smem_desc(base + dg::kW);
+            uint32_t s = 0, full_parity = 0, set = 0, free_parity = 1, half = bar_set, unit = 0;
+            for (uint32_t u; (u = s_list.number(unit)) < u_end; ++unit) {
+                const uint32_t tiles = tiles_of(s_list.at(u)), place = unit & 1u;
+                wait_bar(bar_xfull + 8 * place, (unit / 2) & 1u);
+                for (uint32_t i = 0; i < tiles; ++i) {
+                    for (uint32_t kb = 0; kb < KB; ++kb) {
+                        wait_bar(bar_full + 8 * s, full_parity);
+                        wait_bar(bar_free + 8 * set, free_parity);
+                        umma::fence_after_sync();
+                        const uint64_t da = dx0 + (place * dg::kX + kb * 16384u) / 16, db = dw0 + s * 1024u;
+                        if (leader) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) mma_e4m3_ss<1>(tmem + set * 128u, da + 2 * j, db + 2 * j, idesc, j != 0);
+                            umma::commit(half + 8 * set);
+                            umma::commit(bar_empty + 8 * s);
+                        }
+                        __syncwarp();
+                        if (++s == dg::kStages) { s = 0; full_parity ^= 1u; }
+                        if (++set == dg::kSets) { set = 0; free_parity ^= 1u; }
+                    }
+                    half = 2 * bar_set + 8 * dg::kSets - half;   // the other half's barriers
+                }
+                if (leader) umma::commit(bar_xempty + 8 * place);
+                __syncwarp();
+            }
+            // (the last arrivals are in)
+            for (uint32_t i = unit > 2 ? unit - 2 : 0; i < unit; ++i) wait_bar(bar_xempty + 8 * (i & 1u), (i / 2) & 1u);
         }
     }
     umma::fence_before_sync();
@@ -1024,20 +1297,41 @@ cudaError_t pairs_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     const uint64_t rows = (uint64_t)(kGrouped ? a.n_experts : 1u) * a.M;
     CUtensorMap m0, m1;
     if (rows > 0x7FFFFFFFu || !fp8_map(&m0, a.w[0], rows, a.K, 128) || !fp8_map(&m1, kGateUp ? a.w[1] : a.w[0], rows, a.K, 128)) return cudaErrorInvalidValue;
-    Fp8Args b = a;
-    b.vec = a.M % 4 == 0 && ((uintptr_t)a.out & 15u) == 0;
     const uint64_t per = kGateUp ? (a.M + 127) / 128 : (a.M + 255) / 256, pairs = kGrouped ? (uint64_t)a.n * a.n_used : a.n;
     const uint64_t runs = kGrouped ? (pairs < a.n_experts ? pairs : pairs / 128 + a.n_experts) : (pairs + 127) / 128, units = per * runs;
-    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_pairs_kernel<MODE>, dim3((uint32_t)(units < n_sms ? units : n_sms)), dim3(pg::kThreads), pg::kSmem, b, m0, m1);
+    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_pairs_kernel<MODE>, dim3((uint32_t)(units < n_sms ? units : n_sms)), dim3(pg::kThreads), pg::kSmem, a, m0, m1);
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int MODE>
+cudaError_t down_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
+    constexpr bool kGrouped = MODE == kFp8Down;
+    if (const cudaError_t e = allow_dynamic_smem<fp8_down_kernel<MODE>>((int)dg::kSmem)) return e;
+    if (const cudaError_t e = check_registers<fp8_down_kernel<MODE>, pg::kRegLaunch>()) return e;
+    const uint64_t rows = (uint64_t)(kGrouped ? a.n_experts : 1u) * a.M;
+    CUtensorMap map;
+    if (rows > 0x7FFFFFFFu || !fp8_map(&map, a.w[0], rows, a.K, 128)) return cudaErrorInvalidValue;
+    const uint64_t per = (a.M + dg::kRows - 1) / dg::kRows, pairs = kGrouped ? (uint64_t)a.n * a.n_used : a.n;
+    const uint64_t runs = kGrouped ? (pairs < a.n_experts ? pairs : pairs / 128 + a.n_experts) : (pairs + 127) / 128, units = per * runs;
+    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_down_kernel<MODE>, dim3((uint32_t)(units < n_sms ? units : n_sms)), dim3(pg::kThreads), dg::kSmem, a, map);
+    L.count();
+    return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+// Products of many rows with the rows as lanes
+template <int MODE>
+cudaError_t many_rows(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
+    if constexpr (MODE == kFp8Down || MODE == kFp8SharedDown)
+        if (a.K <= 128 * dg::kMaxBlocks) return down_launch<MODE>(L, a, n_sms);
+    return pairs_launch<MODE>(L, a, n_sms);
 }
 
 template <int MODE>
 cudaError_t group_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
     const uint64_t mean = kGrouped ? (uint64_t)a.n * a.n_used / a.n_experts : a.n;
-    return mean > 24 ? pairs_launch<MODE>(L, a, n_sms) : group_launch<MODE, 32>(L, a, n_sms);
+    return mean > 24 ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE, 32>(L, a, n_sms);
 }
 
 // Which kernel a dense product takes: the least of these estimates, in us, fitted to measurements from 1 to 4096 rows, 1000 to 151,936 weight rows and K = 1040 to 4096.
@@ -1077,8 +1371,8 @@ cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint
         case kFp8Dense: return dense_any(L, a, n_sms);
         case kFp8GateUp: return group_any<kFp8GateUp>(L, a, n_sms);
         case kFp8Down: return group_any<kFp8Down>(L, a, n_sms);
-        case kFp8SharedGateUp: if (a.n > 64) return pairs_launch<kFp8SharedGateUp>(L, a, n_sms); break;
-        case kFp8SharedDown: if (a.n > 64) return pairs_launch<kFp8SharedDown>(L, a, n_sms); break;
+        case kFp8SharedGateUp: if (a.n > 64) return many_rows<kFp8SharedGateUp>(L, a, n_sms); break;
+        case kFp8SharedDown: if (a.n > 64) return many_rows<kFp8SharedDown>(L, a, n_sms); break;
     }
     return launch_fp8_rows(L, mode, a, n_sms);
 }

@@ -321,3 +321,35 @@ def test_no_tokens_and_no_pairs(pkg):
         c.sync()
         assert np.all(d_out.download(np.float32, 5 * 2 * 256) == 9.5)
         _free(w, out, d_off, d_out)
+
+
+@pytest.mark.parametrize("T,E,k,D,F", [(700, 8, 4, 2048, 256), (700, 8, 4, 2048, 512), (500, 6, 4, 2048, 768), (400, 4, 4, 1280, 1280), (1500, 16, 2, 1024, 512), (60, 8, 4, 2048, 512)])
+def test_experts_many_units(pkg, T, E, k, D, F):
+    """Several units a block, sums of one to ten column blocks: the barriers go through many phases.  Twice: the results are the same to the bit."""
+    rng = np.random.default_rng(T + F)
+    dims = pkg.synth.Dims(n_embd=D, n_ff=F, n_expert=E, n_used=k)
+    sel, offsets, pairs = _selection(rng, T, E, k, 0.2)
+    q, s = ref.quantize(rng.standard_normal((T, D)).astype(np.float32))
+    hq, hs = ref.quantize(rng.standard_normal((T * (k + 1), F)).astype(np.float32))
+    (g, gs), (u, us), (d, ds) = (ref.weights(rng, *shape, mats=E) for shape in ((F, D), (F, D), (D, F)))
+    h, contrib = [], []
+    with pkg.Context(dims, n_layer=1, max_tokens=1, device=0) as c:
+        dev = _dev(c, g, gs, u, us, q, s, offsets, pairs, d, ds, hq, hs, sel)
+        for _ in range(2):
+            out = _dev(c, np.full((T, k + 1, F), 9.5, np.float32), np.full((T, k, D), 9.5, np.float32))
+            c.moe_gateup_grouped_fp8(*dev[:8], out[0], T)
+            c.moe_down_grouped_fp8(*dev[8:12], dev[12], dev[6], dev[7], out[1], T)
+            c.sync()
+            h.append(out[0].download(np.float32, (T, k + 1, F)))
+            contrib.append(out[1].download(np.float32, (T, k, D)))
+            _free(*out)
+        _free(*dev)
+    assert np.array_equal(h[0], h[1]) and np.array_equal(contrib[0], contrib[1]) and np.all(h[0][:, k] == 9.5)
+    for e in range(E):
+        t, j = (pairs[offsets[e]:offsets[e + 1]] >> 4).astype(int), (pairs[offsets[e]:offsets[e + 1]] & 15).astype(int)
+        (wg, bg), (wu, bu) = (ref.product(m[e], ms[e], q[t], s[t]) for m, ms in ((g, gs), (u, us)))
+        assert np.all(np.abs(h[0][t, j] - _silu(wg) * wu) <= _swiglu_bound(wg, wu, bg, bu)), e
+        r = t * (k + 1) + j
+        wd, bd = ref.product(d[e], ds[e], hq[r], hs[r])
+        w = sel["w"][t, j].astype(np.float64)[:, None]
+        assert np.all(np.abs(contrib[0][t, j] - w * wd) <= w * bd + 2.0**-23 * np.abs(w * wd)), e
