@@ -372,25 +372,28 @@ struct GroupUnit { uint32_t e, m0, p0, n; };     // expert, first weight row, fi
 
 // The units of a product: experts that have pairs (of a dense product or the shared expert the one matrix), their runs of pairs cut into parts of PART at most,
 // every part with all row units of the expert; the parts of a row unit next to one another.
-// SORTED: parts of one expert of the same length, experts in descending order of it, units handed out to and fro, so that every block gets as much as the others (with units
-// of 4 to 128 pairs dealt in the experts' order the busiest SM had 1.4 times the average).
-template <int MODE, int PART, uint32_t ROWS, bool SORTED>
+template <int MODE, int PART, uint32_t ROWS>
 struct UnitList {
     static constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
     static constexpr uint32_t kMax = kGrouped ? gg::kMaxExperts : 1u;
     uint32_t unit[kMax + 1], p0[kMax], p1[kMax];     // per live expert: first unit, run
     uint32_t scan[16][2], n_live, n_units;
     uint16_t expert[kMax];
-    uint32_t size[SORTED && kGrouped ? kMax / 4 : 1];   // a byte an expert: length of its parts
 
-    static __device__ __forceinline__ uint32_t part_size(uint32_t run) {
-        if (!SORTED || run <= (uint32_t)PART) return SORTED ? run : (uint32_t)PART;
-        const uint32_t parts = (run + PART - 1) / PART;
-        return ((run + parts - 1) / parts + 3u) & ~3u;
-    }
-    // inclusive sums over the block's threads of two numbers
-    __device__ __forceinline__ void sums(uint32_t& c, uint32_t& v) {
-        const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    // by all threads of the block (256 or more; two experts each); __syncthreads behind it
+    __device__ __forceinline__ void make(const Fp8Args& a) {
+        const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, row_units = (a.M + ROWS - 1) / ROWS;
+        uint32_t q0[2] = {}, q1[2] = {}, units[2], c = 0, v = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t e = 2 * tid + i;
+            if (kGrouped) { if (e < a.n_experts) fp8_run(a, e, q0[i], q1[i]); }
+            else if (e == 0) q1[i] = a.n;
+            units[i] = (q1[i] - q0[i] + PART - 1) / PART * row_units;
+            c += units[i] ? 1u : 0u;
+            v += units[i];
+        }
+        const uint32_t c_mine = c, v_mine = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t c1 = __shfl_up_sync(0xFFFFFFFFu, c, o), v1 = __shfl_up_sync(0xFFFFFFFFu, v, o);
@@ -399,74 +402,17 @@ struct UnitList {
         if (lane == 31) { scan[warp][0] = c; scan[warp][1] = v; }
         __syncthreads();
         for (uint32_t w = 0; w < warp; ++w) { c += scan[w][0]; v += scan[w][1]; }
-    }
-    // by all threads of the block (256 or more; two experts each); __syncthreads behind it
-    __device__ __forceinline__ void make(const Fp8Args& a) {
-        const uint32_t tid = threadIdx.x, row_units = (a.M + ROWS - 1) / ROWS;
-        uint32_t q0[2] = {}, q1[2] = {}, units[2], e[2] = {2 * tid, 2 * tid + 1}, c = 0, v = 0;
+        if (tid == blockDim.x - 1) { n_live = c; n_units = v; unit[c] = v; }
+        c -= c_mine; v -= v_mine;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (kGrouped) { if (e[i] < a.n_experts) fp8_run(a, e[i], q0[i], q1[i]); }
-            else if (e[i] == 0) q1[i] = a.n;
-        }
-        if constexpr (SORTED && kGrouped) {
-            uint8_t* s = reinterpret_cast<uint8_t*>(size);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (e[i] < kMax) s[e[i]] = (uint8_t)part_size(q1[i] - q0[i]);
-            __syncthreads();
-            // an expert's place: how many have longer parts, or as long ones and a lower number
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (q1[i] <= q0[i]) continue;
-                const uint32_t mine = s[e[i]] * 0x01010101u;
-                uint32_t at = 0;
-                for (uint32_t w = 0; w < (a.n_experts + 3) / 4; ++w) {
-                    const uint32_t longer = __vcmpgtu4(size[w], mine), same = __vcmpeq4(size[w], mine);
-                    const uint32_t before = w < e[i] / 4 ? 0xFFFFFFFFu : w > e[i] / 4 ? 0u : (1u << (8 * (e[i] & 3u))) - 1u;
-                    at += __popc(longer | (same & before));
-                }
-                at >>= 3;
-                expert[at] = (uint16_t)e[i]; p0[at] = q0[i]; p1[at] = q1[i];
+        for (int i = 0; i < 2; ++i)
+            if (units[i]) {
+                expert[c] = (uint16_t)(2 * tid + i); p0[c] = q0[i]; p1[c] = q1[i]; unit[c] = v;
                 ++c;
-            }
-            c = __syncthreads_count(c > 0) + __syncthreads_count(c > 1);   // live experts
-            if (tid == 0) n_live = c;
-            const uint32_t live = c;
-            c = 0;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                units[i] = e[i] < live ? (p1[e[i]] - p0[e[i]] + PART - 1) / PART * row_units : 0u;
                 v += units[i];
             }
-            const uint32_t mine = v;
-            sums(c, v);
-            if (tid == blockDim.x - 1) { n_units = v; unit[live] = v; }
-            v -= mine;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (e[i] < live) { unit[e[i]] = v; v += units[i]; }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                units[i] = (q1[i] - q0[i] + PART - 1) / PART * row_units;
-                c += units[i] ? 1u : 0u;
-                v += units[i];
-            }
-            const uint32_t c_mine = c, v_mine = v;
-            sums(c, v);
-            if (tid == blockDim.x - 1) { n_live = c; n_units = v; unit[c] = v; }
-            c -= c_mine; v -= v_mine;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (units[i]) {
-                    expert[c] = (uint16_t)e[i]; p0[c] = q0[i]; p1[c] = q1[i]; unit[c] = v;
-                    ++c;
-                    v += units[i];
-                }
-        }
     }
-    // number of this block's r-th unit, dealt to and fro; n_units or more: none
+    // number of this block's r-th unit, dealt to and fro (the row units of an expert at the same time in neighbouring blocks); n_units or more: none
     __device__ __forceinline__ uint32_t number(uint32_t r) const { return r * gridDim.x + (r & 1u ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
     // position in the list of the expert that unit u belongs to
     __device__ __forceinline__ uint32_t find(uint32_t u) const {
@@ -484,12 +430,12 @@ struct UnitList {
         return of(u, i);
     }
     __device__ __forceinline__ GroupUnit of(uint32_t u, uint32_t i) const {
-        const uint32_t run = p1[i] - p0[i], len = part_size(run), parts = (run + len - 1) / len, k = u - unit[i], ru = k / parts, part = k - ru * parts;
+        const uint32_t run = p1[i] - p0[i], parts = (run + PART - 1) / PART, k = u - unit[i], ru = k / parts, part = k - ru * parts;
         GroupUnit g;
         g.e = kGrouped ? expert[i] : 0u;
         g.m0 = ru * ROWS;
-        g.p0 = p0[i] + part * len;
-        g.n = min(len, run - part * len);
+        g.p0 = p0[i] + part * PART;
+        g.n = min((uint32_t)PART, run - part * PART);
         return g;
     }
 };
@@ -531,7 +477,7 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     extern __shared__ uint8_t smem_dyn[];
     __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets + 2 * gg::kScales + gg::kMeta];
     __shared__ uint32_t s_tmem;
-    __shared__ UnitList<MODE, NT, kGateUp ? 128u : 256u, false> s_list;
+    __shared__ UnitList<MODE, NT, kGateUp ? 128u : 256u> s_list;
     __shared__ uint64_t s_out[gg::kMeta][NT];        // per unit: where a column's results go, ~0: nowhere; its routing weight
     __shared__ float s_wt[gg::kMeta][NT];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
@@ -809,7 +755,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     extern __shared__ uint8_t smem_dyn[];
     __shared__ __align__(8) unsigned long long s_bar[2 * pg::kStages + 4];
     __shared__ uint32_t s_tmem;
-    __shared__ UnitList<MODE, 128, kGateUp ? 128u : 256u, true> s_list;
+    __shared__ UnitList<MODE, 128, kGateUp ? 128u : 256u> s_list;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
     const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * pg::kStages, bar_set = bar_empty + 8 * pg::kStages, bar_free = bar_set + 16;
@@ -1022,7 +968,7 @@ fp8_down_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map) {
     extern __shared__ uint8_t smem_dyn[];
     __shared__ __align__(8) unsigned long long s_bar[4 + 2 * dg::kStages + 3 * dg::kSets];
     __shared__ uint32_t s_tmem;
-    __shared__ UnitList<MODE, 128, dg::kRows, true> s_list;
+    __shared__ UnitList<MODE, 128, dg::kRows> s_list;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
     const uint32_t bar_xfull = smem_addr(s_bar), bar_xempty = bar_xfull + 16, bar_full = bar_xempty + 16, bar_empty = bar_full + 8 * dg::kStages;
@@ -1327,11 +1273,14 @@ cudaError_t many_rows(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     return pairs_launch<MODE>(L, a, n_sms);
 }
 
+// Pairs an expert, on average, from which they are the lanes: gate/up of 2048 tokens (64) 162 us as columns, 135 as lanes, of 1024 113 and 124; down 112, 108 and 73, 96.
+constexpr uint64_t kManyPairs = 44;
+
 template <int MODE>
 cudaError_t group_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
     const uint64_t mean = kGrouped ? (uint64_t)a.n * a.n_used / a.n_experts : a.n;
-    return mean > 24 ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE, 32>(L, a, n_sms);
+    return mean > kManyPairs ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE, 32>(L, a, n_sms);
 }
 
 // Which kernel a dense product takes: the least of these estimates, in us, fitted to measurements from 1 to 4096 rows, 1000 to 151,936 weight rows and K = 1040 to 4096.

@@ -353,3 +353,152 @@ def test_experts_many_units(pkg, T, E, k, D, F):
         wd, bd = ref.product(d[e], ds[e], hq[r], hs[r])
         w = sel["w"][t, j].astype(np.float64)[:, None]
         assert np.all(np.abs(contrib[0][t, j] - w * wd) <= w * bd + 2.0**-23 * np.abs(w * wd)), e
+
+
+@pytest.mark.parametrize("n", [1, 24, 300])
+def test_gemm_beyond_32_bits(ctx, n):
+    """A matrix of more than 2^32 bytes: rows at both ends and across the 4 GB line."""
+    import torch
+    M, K = (1 << 20) + 37, 4112
+    w = torch.randint(0, 120, (M, K), dtype=torch.uint8, device="cuda")
+    ws = torch.rand((ref.blocks(M), ref.blocks(K)), device="cuda")
+    rng = np.random.default_rng(n)
+    q, s = ref.quantize(rng.standard_normal((n, K)).astype(np.float32))
+    d_q, d_s = torch.from_numpy(q).cuda(), torch.from_numpy(s).cuda()
+    y = torch.empty((n, M), device="cuda")
+    torch.cuda.synchronize()
+    ctx.fp8_gemm(w, ws, d_q, d_s, y, M, K, n)
+    ctx.sync()
+    line = (1 << 32) // K // 128 * 128
+    for r0 in (0, line - 128, line, (M - 1) // 128 * 128):
+        rows = slice(r0, min(r0 + 128, M))
+        want, bound = ref.product(w[rows].cpu().numpy(), ws[r0 // 128:r0 // 128 + 1].cpu().numpy(), q, s)
+        assert np.all(np.abs(y[:, rows].cpu().numpy() - want) <= bound), r0
+
+
+def test_misaligned_results_are_refused(pkg):
+    dims = pkg.synth.Dims(n_embd=256, n_ff=256, n_expert=4, n_used=2)
+    with pkg.Context(dims, n_layer=1, max_tokens=1, device=0) as c:
+        d = c.alloc(1 << 20)
+        for bad in (lambda: c.moe_gateup_grouped_fp8(d, d, d, d, d, d, d, d, d.ptr + 4, 1), lambda: c.moe_down_grouped_fp8(d, d, d, d, d, d, d, d.ptr + 8, 1),
+                    lambda: c.moe_shared_gateup_fp8(d, d, d, d, d, d, d.ptr + 12, 1), lambda: c.moe_shared_down_fp8(d, d, d, d, d, d.ptr + 4, 1),
+                    lambda: c.moe_gateup_grouped_fp8(d.ptr + 1, d, d, d, d, d, d, d, d, 1), lambda: c.moe_down_grouped_fp8(d, d, d.ptr + 8, d, d, d, d, d, 1),
+                    lambda: c.moe_gateup_grouped_fp8(d, d, d, d, d, d, None, d, d, 1)):
+            with pytest.raises(pkg.QkmError) as ei:
+                bad()
+            assert ei.value.code == -1
+        with pytest.raises(pkg.QkmError) as ei:
+            c.moe_down_grouped_fp8(d, d, d, d, d, d, d, d, 1 << 27)
+        assert ei.value.code == -3
+        d.free()
+
+
+@pytest.mark.parametrize("T", [3, 60, 400])
+def test_captured_and_replayed_on_a_stream(pkg, T):
+    """The whole chain of an FP8 layer on a stream of the caller's, captured once and replayed on other inputs: the bits of the eager calls."""
+    import torch
+    E, k, D, F = 8, 4, 512, 512
+    rng = np.random.default_rng(T)
+    dims = pkg.synth.Dims(n_embd=D, n_ff=F, n_expert=E, n_used=k)
+    sel, offsets, pairs = _selection(rng, T, E, k)
+    mats = [t for shape in ((F, D), (F, D), (D, F)) for t in ref.weights(rng, *shape, mats=E)]
+    dev = [torch.from_numpy(np.ascontiguousarray(a).view(np.uint8).reshape(-1)).cuda() for a in (*mats, sel, offsets, pairs)]
+    g, gs, u, us, d, ds, d_sel, d_off, d_pairs = dev
+    xs = [torch.from_numpy(rng.standard_normal((T, D)).astype(np.float32)).cuda() for _ in range(2)]
+    x, logits = torch.empty_like(xs[0]), torch.randn((T, E), device="cuda")
+    q, s = torch.empty((T, D), dtype=torch.uint8, device="cuda"), torch.empty((T, D // 128), device="cuda")
+    hq, hs = torch.empty((T * (k + 1), F), dtype=torch.uint8, device="cuda"), torch.empty((T * (k + 1), F // 128), device="cuda")
+    h, contrib = torch.zeros((T, k + 1, F), device="cuda"), torch.zeros((T, k, D), device="cuda")
+    y, counts, probs, loss, grad = torch.zeros((T, F), device="cuda"), torch.zeros(E + 1, dtype=torch.int32, device="cuda"), torch.zeros(E, device="cuda"), torch.zeros(1, device="cuda"), torch.zeros((T, E), device="cuda")
+    st = torch.cuda.Stream()
+    with pkg.Context(dims, n_layer=1, max_tokens=1, device=0) as c:
+        c.set_stream(st.cuda_stream)
+
+        def chain():
+            c.moe_balance(logits, d_sel, None, T, 0.01, counts, probs, loss)
+            c.moe_balance_grad(logits, None, counts, T, 0.01, None, grad)
+            c.fp8_quantize(x, T, D, q, s)
+            c.fp8_gemm(g, gs, q, s, y, F, D, T)
+            c.moe_gateup_grouped_fp8(g, gs, u, us, q, s, d_off, d_pairs, h, T)
+            c.fp8_quantize(h, T * (k + 1), F, hq, hs)
+            c.moe_down_grouped_fp8(d, ds, hq, hs, d_sel, d_off, d_pairs, contrib, T)
+
+        outs, graph = [], torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            for xi in xs:
+                x.copy_(xi)
+                chain()
+                outs.append([t.clone() for t in (y, h, contrib, loss, counts, grad)])
+            st.synchronize()
+            with torch.cuda.graph(graph, stream=st):
+                chain()
+            for xi, want in zip(xs, outs):
+                for t in (y, h, contrib, loss, counts, grad):
+                    t.zero_()
+                x.copy_(xi)
+                graph.replay()
+                for t, w in zip((y, h, contrib, loss, counts, grad), want):
+                    assert torch.equal(t, w)
+            st.synchronize()
+        c.sync()
+        del graph
+
+
+def test_layer_chain(pkg):
+    """The operators as a layer uses them: router logits and selection, load, pairs by expert, FP8 gate/up and down of routed and shared experts, the fold with
+    the residual and the norm.  Each stage against 64 bits from what the stage before gave."""
+    from qwen_kernel_b200 import SEL_DTYPE
+    T, E, k, D, F = 70, 16, 4, 512, 256
+    rng = np.random.default_rng(1)
+    dims = pkg.synth.Dims(n_embd=D, n_ff=F, n_expert=E, n_used=k)
+    x = rng.standard_normal((T, D)).astype(np.float32)
+    resid = rng.standard_normal((T, D)).astype(np.float32)
+    router = (rng.standard_normal((E, D)) * 0.05).astype(np.float32)
+    gis, norm = (rng.standard_normal(D) * 0.05).astype(np.float32), np.ones(D, np.float32)
+    routed = [ref.weights(rng, *shape, mats=E) for shape in ((F, D), (F, D), (D, F))]
+    shared = [ref.weights(rng, *shape) for shape in ((F, D), (F, D), (D, F))]
+    with pkg.Context(dims, n_layer=1, max_tokens=T, device=0) as c:
+        d_x, d_resid, d_router, d_gis, d_norm = _dev(c, x, resid, router, gis, norm)
+        d_logits, d_sel, d_off, d_pairs = c.alloc(T * E * 4), c.alloc(T * 160), c.alloc((E + 1) * 4), c.alloc(T * k * 4)
+        d_counts, d_probs, d_loss = c.alloc((E + 1) * 4), c.alloc(E * 4), c.alloc(4)
+        d_q, d_s, d_h = c.alloc(T * D), c.alloc(T * D // 128 * 4), c.alloc(T * (k + 1) * F * 4)
+        d_hq, d_hs, d_contrib, d_y2 = c.alloc(T * (k + 1) * F), c.alloc(T * (k + 1) * F // 128 * 4), c.alloc(T * k * D * 4), c.alloc(T * D * 4)
+        d_out, d_xn = c.alloc(T * D * 4), c.alloc(T * D * 4)
+        (g, gs), (u, us), (d, ds) = [_dev(c, *m) for m in routed]
+        (sg, sgs), (su, sus), (sd, sds) = [_dev(c, *m) for m in shared]
+        c.moe_logits(0, d_router, d_x, d_logits, T)
+        c.moe_select(d_logits, d_gis, d_x, d_sel, T)
+        c.moe_balance(d_logits, d_sel, None, T, 1.0, d_counts, d_probs, d_loss)
+        c.moe_group_pairs(d_sel, T, d_off, d_pairs)
+        c.fp8_quantize(d_x, T, D, d_q, d_s)
+        c.moe_gateup_grouped_fp8(g, gs, u, us, d_q, d_s, d_off, d_pairs, d_h, T)
+        c.moe_shared_gateup_fp8(sg, sgs, su, sus, d_q, d_s, d_h, T)
+        c.fp8_quantize(d_h, T * (k + 1), F, d_hq, d_hs)
+        c.moe_down_grouped_fp8(d, ds, d_hq, d_hs, d_sel, d_off, d_pairs, d_contrib, T)
+        c.moe_shared_down_fp8(sd, sds, d_hq, d_hs, d_sel, d_y2, T)
+        c.add_rms3_grouped(d_resid, d_contrib, d_y2, d_norm, d_out, d_xn, T, D, k)
+        c.sync()
+        sel, off, counts = d_sel.download(SEL_DTYPE, T), d_off.download(np.uint32, E + 1), d_counts.download(np.uint32, E + 1)
+        h, contrib = d_h.download(np.float32, (T, k + 1, F)), d_contrib.download(np.float32, (T, k, D))
+        y2, out, loss = d_y2.download(np.float32, (T, D)), d_out.download(np.float32, (T, D)), d_loss.download(np.float32, 1)[0]
+    assert np.array_equal(counts[:E], np.diff(off)) and counts[E] == T       # the load is what the pairs were grouped by
+    logits = x.astype(np.float64) @ router.astype(np.float64).T
+    p = np.exp(logits - logits.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    assert abs(loss - E / (T * k) * (counts[:E] * p.mean(0)).sum()) < 1e-4
+    q, s = ref.quantize(x)
+    hq, hs = ref.quantize(h.reshape(-1, F))
+    for e in range(E + 1):
+        t, j = np.nonzero(sel["ids"][:, :k] == e) if e < E else (np.arange(T), np.full(T, k))
+        if t.size == 0:
+            continue
+        m = [(w[e], ws[e]) for w, ws in routed] if e < E else shared
+        (wg, bg), (wu, bu) = ref.product(*m[0], q[t], s[t]), ref.product(*m[1], q[t], s[t])
+        assert np.all(np.abs(h[t, j] - _silu(wg) * wu) <= _swiglu_bound(wg, wu, bg, bu)), e
+        wd, bd = ref.product(*m[2], hq[t * (k + 1) + j], hs[t * (k + 1) + j])
+        w = (sel["w"][t, j] if e < E else sel["w_shared"][t]).astype(np.float64)[:, None]
+        got = contrib[t, j] if e < E else y2
+        assert np.all(np.abs(got - w * wd) <= w * bd + 2.0**-23 * np.abs(w * wd)), e
+    fold = resid.astype(np.float64) + contrib.sum(1, dtype=np.float64) + y2
+    assert np.all(np.abs(out - fold) <= (k + 3) * 2.0**-23 * (np.abs(resid) + np.abs(contrib).sum(1) + np.abs(y2)))
