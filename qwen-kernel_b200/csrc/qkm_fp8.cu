@@ -100,35 +100,32 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
 
 __device__ __forceinline__ uint4 ld16(const uint8_t* p, bool there) { return there ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0); }
 
-template <int MODE> constexpr int rows_mats() { return MODE == kFp8GateUp || MODE == kFp8SharedGateUp ? 2 : 1; }
+template <int MODE> constexpr int rows_mats() { return MODE == kFp8SharedGateUp ? 2 : 1; }
 
-// U: column blocks that a warp loads ahead of their MMAs.  16 weight rows from m0 of expert e times rows [p0, p0 + 8 NT) of its run; NT: groups of eight rows
+// U: column blocks that a warp loads ahead of their MMAs.  16 weight rows from m0 times rows [p0, p0 + 8 NT); NT: groups of eight rows
 template <int MODE, int NT, int U>
-__device__ __forceinline__ void rows_tile(const Fp8Args& a, uint32_t e, uint32_t m0, uint32_t p0, uint32_t p1, float* s_red) {
+__device__ __forceinline__ void rows_tile(const Fp8Args& a, uint32_t m0, uint32_t p0, float* s_red) {
     constexpr int MATS = rows_mats<MODE>();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u, g = lane >> 2, t = lane & 3u;
-    const uint32_t KB = fp8_blocks(a.K), MB = fp8_blocks(a.M);
+    const uint32_t KB = fp8_blocks(a.K), p1 = a.n;
     const uint8_t* xrow[NT];
     const float* xsc[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        uint64_t o;
-        float w;
         const uint32_t p = p0 + 8 * j + g;
-        const uint32_t r = p < p1 ? fp8_row<MODE>(a, p, o, w) : kFp8NoRow;
-        xrow[j] = r == kFp8NoRow ? nullptr : a.xq + (uint64_t)r * a.K;
+        xrow[j] = p < p1 ? a.xq + (uint64_t)fp8_place<MODE>(a, p).row * a.K : nullptr;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const uint32_t pc = p0 + 8 * j + 2 * t + c, rc = pc < p1 ? fp8_row<MODE>(a, pc, o, w) : kFp8NoRow;
-            xsc[j][c] = rc == kFp8NoRow ? nullptr : a.x_scale + (uint64_t)rc * KB;
+            const uint32_t pc = p0 + 8 * j + 2 * t + c;
+            xsc[j][c] = pc < p1 ? a.x_scale + (uint64_t)fp8_place<MODE>(a, pc).row * KB : nullptr;
         }
     }
     const uint8_t* wrow[MATS];
     const float* wsc[MATS];
 #pragma unroll
     for (int m = 0; m < MATS; ++m) {
-        wrow[m] = a.w[m] + ((uint64_t)e * a.M + m0 + g) * a.K;
-        wsc[m] = a.w_scale[m] + ((uint64_t)e * MB + m0 / 128) * KB;
+        wrow[m] = a.w[m] + (uint64_t)(m0 + g) * a.K;
+        wsc[m] = a.w_scale[m] + (uint64_t)(m0 / 128) * KB;
     }
     const bool has0 = m0 + g < a.M, has1 = m0 + g + 8 < a.M;
     float acc[MATS][NT][4] = {};
@@ -193,34 +190,8 @@ __device__ __forceinline__ void rows_tile(const Fp8Args& a, uint32_t e, uint32_t
 #pragma unroll
         for (int mat = 0; mat < MATS; ++mat)
             for (int w = 0; w < kRowsWarps; ++w) v[mat] += s_red[w * kTile + mat * kCols * 16 + i];
-        uint64_t o;
-        float wt;
-        if (fp8_row<MODE>(a, p, o, wt) == kFp8NoRow) continue;
-        a.out[o * a.M + m] = MATS == 2 ? swiglu(v[0], v[MATS - 1]) : MODE == kFp8Dense ? v[0] : wt * v[0];
+        a.out[fp8_place<MODE>(a, p).out * a.M + m] = MATS == 2 ? swiglu(v[0], v[MATS - 1]) : MODE == kFp8Dense ? v[0] : fp8_weight<MODE>(a, p) * v[0];
     }
-}
-
-// experts that have pairs, in order; returns how many (the same for all threads)
-__device__ __forceinline__ uint32_t live_experts(const Fp8Args& a, uint16_t* s_live) {
-    __shared__ uint32_t s_cnt[kRowsWarps];
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-    uint32_t total = 0;
-    for (uint32_t e0 = 0; e0 < a.n_experts; e0 += kRowsThreads) {
-        const uint32_t e = e0 + tid;
-        uint32_t p0 = 0, p1 = 0;
-        if (e < a.n_experts) fp8_run(a, e, p0, p1);
-        const uint32_t b = __ballot_sync(0xFFFFFFFFu, p1 > p0);
-        if (lane == 0) s_cnt[warp] = __popc(b);
-        __syncthreads();
-        uint32_t at = total;
-        for (uint32_t w = 0; w < kRowsWarps; ++w) {
-            if (w < warp) at += s_cnt[w];
-            total += s_cnt[w];
-        }
-        if (p1 > p0) s_live[at + __popc(b & ((1u << lane) - 1u))] = (uint16_t)e;
-        __syncthreads();
-    }
-    return total;
 }
 
 template <int MODE, int NT, int U>
@@ -228,35 +199,22 @@ __global__ void __launch_bounds__(kRowsThreads)
 fp8_rows_kernel(const Fp8Args a) {
     constexpr uint32_t kCols = 8 * NT;
     __shared__ float s_red[kRowsWarps * rows_mats<MODE>() * kCols * 16];
-    __shared__ uint16_t s_live[512];
     pdl_trigger();
     pdl_wait();
-    const uint32_t tiles = (a.M + 15) / 16;
-    constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
-    const uint64_t units = (uint64_t)tiles * (kGrouped ? live_experts(a, s_live) : 1u);
-    for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const uint32_t i = (uint32_t)(u / tiles), m0 = (uint32_t)(u - (uint64_t)i * tiles) * 16u;
-        uint32_t e = 0, p0 = 0, p1 = a.n;
-        if (kGrouped) { e = s_live[i]; fp8_run(a, e, p0, p1); }
-        for (uint32_t p = p0 + blockIdx.y * kCols; p < p1; p += gridDim.y * kCols) rows_tile<MODE, NT, U>(a, e, m0, p, p1, s_red);
-    }
+    for (uint32_t p = blockIdx.y * kCols; p < a.n; p += gridDim.y * kCols) rows_tile<MODE, NT, U>(a, blockIdx.x * 16u, p, s_red);
 }
 
 template <int MODE>
-cudaError_t rows_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
-    const uint64_t tiles = (a.M + 15) / 16;
-    constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
-    const uint64_t most = kGrouped ? tiles * a.n_experts : tiles;
+cudaError_t rows_launch(const Launch& L, const Fp8Args& a) {
     const Launch P{L.stream, nullptr, true};
-    cudaError_t e;
     auto go = [&](auto kernel, uint32_t cols) {
-        const uint32_t chunks = kGrouped ? 1u : (a.n + cols - 1) / cols;
-        const uint32_t gx = (uint32_t)(kGrouped ? (most < n_sms * 8ull ? most : n_sms * 8ull) : (most < 0x7FFFFFFF ? most : 0x7FFFFFFF));
-        return launch_kernel(P, kernel, dim3(gx, chunks < 65535 ? chunks : 65535), dim3(kRowsThreads), 0, a);
+        const uint32_t chunks = (a.n + cols - 1) / cols;
+        return launch_kernel(P, kernel, dim3((a.M + 15) / 16, chunks < 65535 ? chunks : 65535), dim3(kRowsThreads), 0, a);
     };
-    // As many blocks of columns at once as a warp has (one row, K = 4096, M = 2048: two 6.4 us, four 3.9, 16 rows 7.3 and 5.4; K = 2048, where it has two, four cost occupancy: M = 8192
-    // 6.2 against 9.7)
+    // As many blocks of columns at once as a warp has (one row, K = 4096, M = 2048: two 6.4 us, four 3.9, 16 rows 7.3 and 5.4; K = 2048, where it has two, four cost
+    // occupancy: M = 8192 6.2 against 9.7)
     const bool wide = a.K > 2048;
+    cudaError_t e;
     if (rows_mats<MODE>() == 2) e = a.n <= 8 ? go(fp8_rows_kernel<MODE, 1, 1>, 8) : go(fp8_rows_kernel<MODE, 2, 1>, 16);
     else if (a.n <= 8) e = wide ? go(fp8_rows_kernel<MODE, 1, 4>, 8) : go(fp8_rows_kernel<MODE, 1, 2>, 8);
     else e = wide ? go(fp8_rows_kernel<MODE, 2, 4>, 16) : go(fp8_rows_kernel<MODE, 2, 2>, 16);
@@ -266,17 +224,13 @@ cudaError_t rows_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
 
 }  // namespace
 
-cudaError_t launch_fp8_rows(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) {
-    if (a.n == 0 || a.M == 0) return cudaSuccess;
+cudaError_t launch_fp8_rows(const Launch& L, int mode, const Fp8Args& a) {
     switch (mode) {
-        case kFp8Dense: return rows_launch<kFp8Dense>(L, a, n_sms);
-        case kFp8GateUp: return rows_launch<kFp8GateUp>(L, a, n_sms);
-        case kFp8Down: return rows_launch<kFp8Down>(L, a, n_sms);
-        case kFp8SharedGateUp: return rows_launch<kFp8SharedGateUp>(L, a, n_sms);
-        case kFp8SharedDown: return rows_launch<kFp8SharedDown>(L, a, n_sms);
+        case kFp8Dense: return rows_launch<kFp8Dense>(L, a);
+        case kFp8SharedGateUp: return rows_launch<kFp8SharedGateUp>(L, a);
+        case kFp8SharedDown: return rows_launch<kFp8SharedDown>(L, a);
     }
     return cudaErrorInvalidValue;
 }
-
 
 }  // namespace qkm

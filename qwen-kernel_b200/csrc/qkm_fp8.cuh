@@ -49,14 +49,6 @@ __device__ __forceinline__ float fp8_weight(const Fp8Args& a, uint32_t entry) {
     if (MODE == kFp8Down) return a.sel[entry >> 4].w[entry & 15u];
     return 1.f;
 }
-template <int MODE>
-__device__ __forceinline__ uint32_t fp8_row(const Fp8Args& a, uint32_t p, uint64_t& out_row, float& weight) {
-    const uint32_t entry = MODE == kFp8GateUp || MODE == kFp8Down ? a.pairs[p] : p;
-    const Fp8Place r = fp8_place<MODE>(a, entry);
-    out_row = r.out;
-    weight = r.row == kFp8NoRow ? 0.f : fp8_weight<MODE>(a, entry);
-    return r.row;
-}
 // expert e's run of the list of pairs, whatever the offsets hold inside the list
 __device__ __forceinline__ void fp8_run(const Fp8Args& a, uint32_t e, uint32_t& p0, uint32_t& p1) {
     const uint32_t most = a.n * a.n_used;

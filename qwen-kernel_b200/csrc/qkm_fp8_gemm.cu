@@ -120,6 +120,13 @@ __device__ __forceinline__ void tmem_ld_done(float (&v)[32]) {
                  ::"memory");
 }
 
+// A few polls that end at once when the phase does, then such that let the thread sleep (which take 60 cycles more to wake up); false after about half a second.
+__device__ __forceinline__ bool wait_phase(uint32_t b, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+        if (mbar_try_wait(b, parity)) return true;
+    return mbar_wait_timed(b, parity);
+}
 // whether the phase is through, without waiting for it
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -205,15 +212,7 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
     umma::fence_after_sync();
     const uint32_t tmem = s_tmem;
     Waits waits;
-    // A few polls that end at once when the phase does, then such that let the thread sleep (which take 60 cycles more to wake up).
-    auto wait_bar = [&](uint32_t b, uint32_t parity) {
-        waits.wait([&] {
-#pragma unroll 1
-            for (int i = 0; i < 64; ++i)
-                if (mbar_try_wait(b, parity)) return true;
-            return mbar_wait_timed(b, parity);
-        });
-    };
+    auto wait_bar = [&](uint32_t b, uint32_t parity) { waits.wait([&] { return wait_phase(b, parity); }); };
 
     if (warp >= (uint32_t)tg::kAux) {
         // ---- scale and add: TMEM lanes 32 q .., half h of a set's columns, weight rows of one block of 128
@@ -346,9 +345,9 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
 }
 
 // ---- products grouped by expert (and dense ones of a middling number of rows) --------------------------------------------------
-// Weight rows are the lanes here (M = 128) and a run of at most NT pairs the columns, as many as there are: the weights are what has to be read.  A unit is
+// Weight rows are the lanes here (M = 128) and a run of at most 32 pairs the columns, as many as there are: the weights are what has to be read.  A unit is
 // the gate and the up rows of one 128-row tile, or two tiles of one matrix, times a run; blocks take consecutive units, so that the runs of an expert
-// with more than NT pairs read a tile from the L2.  Weight tiles come by TMA, the rows of the pairs with 16-byte copies, each row's scale of a
+// with more than 32 pairs read a tile from the L2.  Weight tiles come by TMA, the rows of the pairs with 16-byte copies, each row's scale of a
 // column block beside them; the eight warps that scale and add take the row scales from shared memory.
 namespace gg {
 constexpr int kThreads = 512;                    // warps: 0 weights, 1 MMAs, 2 tensor memory, 4 - 7 rows, 8 - 15 scale and add
@@ -356,16 +355,12 @@ constexpr int kRegAux = 40, kRegRows = 72, kRegAdd = 200;
 constexpr int kRegLaunch = 128;
 static_assert(128 * (kRegAux + kRegRows) + 256 * kRegAdd <= kThreads * kRegLaunch, "the shares must not exceed the launch's registers");
 constexpr uint32_t kMaxExperts = 512, kScales = 8, kMeta = 4;   // scale slots; units whose columns' destinations are kept
-template <int NT> struct Tile {
-    static constexpr uint32_t kStage = 2 * 16384 + NT * 128;
-    static constexpr uint32_t kStages = NT > 64 ? 4 : 5;
-    static constexpr uint32_t kSets = NT > 64 ? 2 : 4;                 // of 2 NT columns; fewer than the scale slots less the stages
-    static constexpr uint32_t kSetCols = 512 / kSets;
-    static constexpr uint32_t kScale0 = kStages * kStage;              // [kScales][2][NT] f32: row scale times either matrix's block scale
-    static constexpr uint32_t kSmem = kScale0 + kScales * NT * 8 + 1024;
-    static constexpr int kChunk = NT / 4 < 32 ? NT / 4 : 32;           // columns of a load
-    static constexpr int kChunks = NT / 2 / kChunk;                    // loads a warp and matrix
-};
+constexpr uint32_t kNT = 32, kStage = 2 * 16384 + kNT * 128, kStages = 5;   // columns at most; weights and rows of a column block
+constexpr uint32_t kSets = 4, kSetCols = 512 / kSets;                      // sets of 2 kNT tensor-memory columns
+static_assert(kStages + kSets <= kScales + 2, "a scale slot comes back before its next use is due");
+constexpr uint32_t kScale0 = kStages * kStage;                             // [kScales][2][kNT] f32: row scale times either matrix's block scale
+constexpr uint32_t kSmem = kScale0 + kScales * kNT * 8 + 1024;
+constexpr int kChunk = 8, kChunks = kNT / 2 / kChunk;                      // columns of a load, loads of a warp and matrix
 }  // namespace gg
 
 struct GroupUnit { uint32_t e, m0, p0, n; };     // expert, first weight row, first pair, pairs
@@ -440,11 +435,10 @@ struct UnitList {
     }
 };
 
-__device__ __forceinline__ void tmem_ld8f(uint32_t taddr, float (&v)[8]) {
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, float (&v)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_ld(uint32_t t, float (&v)[8]) { tmem_ld8f(t, v); }
 // waits for the loads, whose registers are used behind it
 template <int N> __device__ __forceinline__ void tmem_done(float (&a)[N], float (&b)[N]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -468,25 +462,23 @@ __device__ __forceinline__ void add4(float* a, const float* v, const uint4& x) {
 // silu(g) * u with the fast division (2 ulp; 0 where e^-g passes 2^126, of a result below 2^-119 |u|)
 __device__ __forceinline__ float silu_times(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
-template <int MODE, int NT>
+template <int MODE>
 __global__ void __launch_bounds__(gg::kThreads, 1)
 fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1) {
-    using T = gg::Tile<NT>;
     constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
-    static_assert(T::kStages + T::kSets <= gg::kScales + 2, "a scale slot comes back before its next use is due");
     extern __shared__ uint8_t smem_dyn[];
-    __shared__ __align__(8) unsigned long long s_bar[2 * T::kStages + 2 * T::kSets + 2 * gg::kScales + gg::kMeta];
+    __shared__ __align__(8) unsigned long long s_bar[2 * gg::kStages + 2 * gg::kSets + 2 * gg::kScales + gg::kMeta];
     __shared__ uint32_t s_tmem;
-    __shared__ UnitList<MODE, NT, kGateUp ? 128u : 256u> s_list;
-    __shared__ uint64_t s_out[gg::kMeta][NT];        // per unit: where a column's results go, ~0: nowhere; its routing weight
-    __shared__ float s_wt[gg::kMeta][NT];
+    __shared__ UnitList<MODE, gg::kNT, kGateUp ? 128u : 256u> s_list;
+    __shared__ uint64_t s_out[gg::kMeta][gg::kNT];        // per unit: where a column's results go, ~0: nowhere; its routing weight
+    __shared__ float s_wt[gg::kMeta][gg::kNT];
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t base = (smem_addr(smem_dyn) + 1023u) & ~1023u;
-    const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * T::kStages, bar_set = bar_empty + 8 * T::kStages, bar_free = bar_set + 8 * T::kSets;
-    const uint32_t bar_sfull = bar_free + 8 * T::kSets, bar_sfree = bar_sfull + 8 * gg::kScales, bar_meta = bar_sfree + 8 * gg::kScales;
+    const uint32_t bar_full = smem_addr(s_bar), bar_empty = bar_full + 8 * gg::kStages, bar_set = bar_empty + 8 * gg::kStages, bar_free = bar_set + 8 * gg::kSets;
+    const uint32_t bar_sfull = bar_free + 8 * gg::kSets, bar_sfree = bar_sfull + 8 * gg::kScales, bar_meta = bar_sfree + 8 * gg::kScales;
     if (tid == 0) {
-        for (uint32_t i = 0; i < T::kStages; ++i) { mbar_init(bar_full + 8 * i, 1 + 4); mbar_init(bar_empty + 8 * i, 1); }
-        for (uint32_t i = 0; i < T::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, 8); }
+        for (uint32_t i = 0; i < gg::kStages; ++i) { mbar_init(bar_full + 8 * i, 1 + 4); mbar_init(bar_empty + 8 * i, 1); }
+        for (uint32_t i = 0; i < gg::kSets; ++i) { mbar_init(bar_set + 8 * i, 1); mbar_init(bar_free + 8 * i, 8); }
         for (uint32_t i = 0; i < gg::kScales; ++i) { mbar_init(bar_sfull + 8 * i, 4); mbar_init(bar_sfree + 8 * i, 8); }
         for (uint32_t i = 0; i < gg::kMeta; ++i) mbar_init(bar_meta + 8 * i, 8);
         mbar_fence_init();
@@ -504,14 +496,7 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     uint32_t live_i = s_list.find(u_first);
     auto unit_of = [&](uint32_t u, uint32_t& i) -> GroupUnit { return s_list.at(u, i); };
     Waits waits;
-    auto wait_bar = [&](uint32_t b, uint32_t parity) {
-        waits.wait([&] {
-#pragma unroll 1
-            for (int i = 0; i < 64; ++i)
-                if (mbar_try_wait(b, parity)) return true;
-            return mbar_wait_timed(b, parity);
-        });
-    };
+    auto wait_bar = [&](uint32_t b, uint32_t parity) { waits.wait([&] { return wait_phase(b, parity); }); };
 
     if (warp >= 8) {
         // ---- scale and add
@@ -520,45 +505,45 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
         uint32_t blk = 0, set = 0, set_parity = 0, meta = 0;
         for (uint32_t u = u_first; u < u_end; ++u, meta = (meta + 1) % gg::kMeta) {
             const GroupUnit g = unit_of(u, live_i);
-            float acc[2][T::kChunks][T::kChunk];
+            float acc[2][gg::kChunks][gg::kChunk];
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int j = 0; j < T::kChunks; ++j)
+                for (int j = 0; j < gg::kChunks; ++j)
 #pragma unroll
-                    for (int i = 0; i < T::kChunk; ++i) acc[m][j][i] = 0.f;
+                    for (int i = 0; i < gg::kChunk; ++i) acc[m][j][i] = 0.f;
             for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
-                const uint32_t slot = blk % gg::kScales, sc = base + T::kScale0 + slot * NT * 8, t = tmem + ((32 * q) << 16) + set * T::kSetCols;
+                const uint32_t slot = blk % gg::kScales, sc = base + gg::kScale0 + slot * gg::kNT * 8, t = tmem + ((32 * q) << 16) + set * gg::kSetCols;
                 wait_bar(lane == 1 ? bar_sfull + 8 * slot : bar_set + 8 * set, lane == 1 ? (blk / gg::kScales) & 1u : set_parity);   // two barriers in one poll
                 __syncwarp();
                 umma::fence_after_sync();
 #pragma unroll
-                for (int j = 0; j < T::kChunks; ++j) {
-                    const uint32_t col = (2 * j + h) * T::kChunk;
+                for (int j = 0; j < gg::kChunks; ++j) {
+                    const uint32_t col = (2 * j + h) * gg::kChunk;
                     if (col >= g.n) continue;
-                    float v0[T::kChunk], v1[T::kChunk];
+                    float v0[gg::kChunk], v1[gg::kChunk];
                     tmem_ld(t + col, v0);
-                    tmem_ld(t + NT + col, v1);
+                    tmem_ld(t + gg::kNT + col, v1);
                     tmem_done(v0, v1);
 #pragma unroll
-                    for (int i = 0; i < T::kChunk; i += 4) {
+                    for (int i = 0; i < gg::kChunk; i += 4) {
                         add4(&acc[0][j][i], &v0[i], lds128(sc + 4 * (col + i)));
-                        add4(&acc[1][j][i], &v1[i], lds128(sc + 4 * (NT + col + i)));
+                        add4(&acc[1][j][i], &v1[i], lds128(sc + 4 * (gg::kNT + col + i)));
                     }
                 }
                 umma::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) { mbar_arrive(bar_free + 8 * set); mbar_arrive(bar_sfree + 8 * slot); }
-                if (++set == T::kSets) { set = 0; set_parity ^= 1u; }
+                if (++set == gg::kSets) { set = 0; set_parity ^= 1u; }
             }
             if (!__any_sync(0xFFFFFFFFu, waits.out)) {
                 const uint32_t m = g.m0 + 32 * q + lane;
                 const bool in0 = m < a.M, in1 = m + 128 < a.M;
 #pragma unroll
-                for (int j = 0; j < T::kChunks; ++j)
+                for (int j = 0; j < gg::kChunks; ++j)
 #pragma unroll
-                    for (int i = 0; i < T::kChunk; ++i) {
-                        const uint32_t col = (2 * j + h) * T::kChunk + i;
+                    for (int i = 0; i < gg::kChunk; ++i) {
+                        const uint32_t col = (2 * j + h) * gg::kChunk + i;
                         if (col >= g.n) continue;
                         const uint64_t at = s_out[meta][col];
                         if (at == ~0ull) continue;
@@ -579,13 +564,13 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
         // ---- rows of the pairs: four rows x 128 columns an instruction; a stage is announced two stages later, so that three are under way.  Beside them,
         // a lane for each column: the scales, multiplied, and where the column's results go.  The list of the next unit's pairs is read a unit ahead.
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(gg::kRegRows));
-        constexpr int kGroups = NT / 16;                 // of four rows, this warp's
+        constexpr int kGroups = gg::kNT / 16;                 // of four rows, this warp's
         const uint32_t w = warp - 4, rr = lane >> 3, ck = lane & 7u, mine = w * 32 + lane;
         uint32_t blk = 0, unit = 0;
         auto announce = [&](uint32_t i) {
             umma::fence_smem_to_async();
             __syncwarp();
-            if (lane == 0) { mbar_arrive(bar_full + 8 * (i % T::kStages)); mbar_arrive(bar_sfull + 8 * (i % gg::kScales)); }
+            if (lane == 0) { mbar_arrive(bar_full + 8 * (i % gg::kStages)); mbar_arrive(bar_sfull + 8 * (i % gg::kScales)); }
         };
         // entry of the list for a column, the last one past the end (nobody looks at those columns)
         auto entry = [&](const GroupUnit& g, uint32_t col) -> uint32_t { const uint32_t p = g.p0 + min(col, g.n - 1); return kGrouped ? a.pairs[p] : p; };
@@ -595,7 +580,7 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
             g = unit_of(u, live_i);
 #pragma unroll
             for (int i = 0; i < kGroups; ++i) pr[i] = entry(g, 16 * i + 4 * w + rr);
-            if (mine < (uint32_t)NT) pr_mine = entry(g, mine);
+            if (mine < gg::kNT) pr_mine = entry(g, mine);
         };
         if (u_first < u_end) entries(u_first);
         bool out = false;
@@ -611,31 +596,31 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
             const float* xs = a.x_scale + (uint64_t)(me.row == kFp8NoRow ? 0u : me.row) * KB;
             const float* ws0 = a.w_scale[0] + ((uint64_t)g.e * MB + g.m0 / 128u) * KB;
             const float* ws1 = kGateUp ? a.w_scale[1] + ((uint64_t)g.e * MB + g.m0 / 128u) * KB : ws0 + (g.m0 / 128u + 1 < MB ? KB : 0u);
-            const float wt = me.row == kFp8NoRow || mine >= (uint32_t)NT ? 0.f : fp8_weight<MODE>(a, pr_mine);
+            const float wt = me.row == kFp8NoRow || mine >= gg::kNT ? 0.f : fp8_weight<MODE>(a, pr_mine);
             float x0 = xs[0], wa0 = ws0[0], wb0 = ws1[0], x1 = KB > 1 ? xs[1] : 0.f, wa1 = KB > 1 ? ws0[1] : 0.f, wb1 = KB > 1 ? ws1[1] : 0.f;
             if (unit >= gg::kMeta) wait_bar(bar_meta + 8 * meta, (unit / gg::kMeta - 1) & 1u);
-            if (mine < (uint32_t)NT) s_out[meta][mine] = mine >= n || me.row == kFp8NoRow ? ~0ull : me.out * a.M;
+            if (mine < gg::kNT) s_out[meta][mine] = mine >= n || me.row == kFp8NoRow ? ~0ull : me.out * a.M;
             if (u + 1 < u_end) entries(u + 1);
             for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
-                const uint32_t s = blk % T::kStages, slot = blk % gg::kScales;
+                const uint32_t s = blk % gg::kStages, slot = blk % gg::kScales;
                 const bool there = kb * 128u + ck * 16u < a.K;
                 const float xc = x0, wac = wa0, wbc = wb0;
                 x0 = x1; wa0 = wa1; wb0 = wb1;
                 if (kb + 2 < KB) { x1 = xs[kb + 2]; wa1 = ws0[kb + 2]; wb1 = ws1[kb + 2]; }
-                if (blk >= T::kStages) wait_bar(bar_empty + 8 * s, (blk / T::kStages - 1) & 1u);
+                if (blk >= gg::kStages) wait_bar(bar_empty + 8 * s, (blk / gg::kStages - 1) & 1u);
                 if (blk >= gg::kScales) wait_bar(bar_sfree + 8 * slot, (blk / gg::kScales - 1) & 1u);
                 if (__any_sync(0xFFFFFFFFu, waits.out)) { out = true; break; }
-                const uint32_t dst = base + s * T::kStage + 32768u;
+                const uint32_t dst = base + s * gg::kStage + 32768u;
 #pragma unroll
                 for (int i = 0; i < kGroups; ++i)
                     if (16u * i < n)
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + umma::sw128_chunk(16 * i + 4 * w + rr, ck)), "l"(there ? src[i] + kb * 128u : a.xq),
                                      "r"(there ? 16u : 0u) : "memory");
                 asm volatile("cp.async.commit_group;" ::: "memory");
-                if (mine < (uint32_t)NT) {
-                    const uint32_t sc = base + T::kScale0 + (slot * 2 * NT + mine) * 4u;
+                if (mine < gg::kNT) {
+                    const uint32_t sc = base + gg::kScale0 + (slot * 2 * gg::kNT + mine) * 4u;
                     asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc), "f"(xc * wac) : "memory");
-                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc + NT * 4u), "f"(xc * wbc) : "memory");
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(sc + gg::kNT * 4u), "f"(xc * wbc) : "memory");
                     if (kb + 1 == KB) s_wt[meta][mine] = wt;
                 }
                 if (blk >= 2) {
@@ -657,8 +642,8 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                 const GroupUnit g = unit_of(u, live_i);
                 const uint32_t r0 = g.e * a.M + g.m0, r1 = kGateUp ? r0 : r0 + 128;
                 for (uint32_t kb = 0; kb < KB; ++kb, ++blk) {
-                    const uint32_t s = blk % T::kStages, dst = base + s * T::kStage, full = bar_full + 8 * s;
-                    if (blk >= T::kStages) wait_bar(bar_empty + 8 * s, (blk / T::kStages - 1) & 1u);
+                    const uint32_t s = blk % gg::kStages, dst = base + s * gg::kStage, full = bar_full + 8 * s;
+                    if (blk >= gg::kStages) wait_bar(bar_empty + 8 * s, (blk / gg::kStages - 1) & 1u);
                     if (__any_sync(0xFFFFFFFFu, waits.out)) { out = true; break; }   // a barrier that still counts bytes takes no second arrival
                     if (lane == 0) {
                         mbar_expect_tx(full, 32768u);
@@ -668,7 +653,7 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                     __syncwarp();
                 }
             }
-            for (uint32_t i = blk > T::kStages ? blk - T::kStages : 0; i < blk && !out; ++i) wait_bar(bar_empty + 8 * (i % T::kStages), (i / T::kStages) & 1u);
+            for (uint32_t i = blk > gg::kStages ? blk - gg::kStages : 0; i < blk && !out; ++i) wait_bar(bar_empty + 8 * (i % gg::kStages), (i / gg::kStages) & 1u);
         } else if (warp == 1) {
             // ---- MMAs
             const bool leader = umma::elect_one();
@@ -685,16 +670,16 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                     if (leader) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            mma_e4m3_ss<1>(tmem + set * T::kSetCols, da + 2 * j, da + 2048 + 2 * j, idesc, j != 0);
-                            mma_e4m3_ss<1>(tmem + set * T::kSetCols + NT, da + 1024 + 2 * j, da + 2048 + 2 * j, idesc, j != 0);
+                            mma_e4m3_ss<1>(tmem + set * gg::kSetCols, da + 2 * j, da + 2048 + 2 * j, idesc, j != 0);
+                            mma_e4m3_ss<1>(tmem + set * gg::kSetCols + gg::kNT, da + 1024 + 2 * j, da + 2048 + 2 * j, idesc, j != 0);
                         }
                         umma::commit(bar_set + 8 * set);
                         umma::commit(bar_empty + 8 * s);
                     }
                     __syncwarp();
-                    da += T::kStage / 16;
-                    if (++s == T::kStages) { s = 0; da = da0; full_parity ^= 1u; }
-                    if (++set == T::kSets) { set = 0; free_parity ^= 1u; }
+                    da += gg::kStage / 16;
+                    if (++s == gg::kStages) { s = 0; da = da0; full_parity ^= 1u; }
+                    if (++set == gg::kSets) { set = 0; free_parity ^= 1u; }
                 }
             }
         }
@@ -775,14 +760,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     const uint32_t tmem = s_tmem, n_units = s_list.n_units;
     const uint32_t u_end = n_units;
     Waits waits;
-    auto wait_bar = [&](uint32_t b, uint32_t parity) {
-        waits.wait([&] {
-#pragma unroll 1
-            for (int i = 0; i < 64; ++i)
-                if (mbar_try_wait(b, parity)) return true;
-            return mbar_wait_timed(b, parity);
-        });
-    };
+    auto wait_bar = [&](uint32_t b, uint32_t parity) { waits.wait([&] { return wait_phase(b, parity); }); };
     // entry of the list of pairs for a row of a unit, the last one past its end (nobody looks at those rows)
     auto entry = [&](const GroupUnit& g, uint32_t row) -> uint32_t { const uint32_t p = g.p0 + min(row, g.n - 1); return kGrouped ? a.pairs[p] : p; };
 
@@ -989,14 +967,7 @@ fp8_down_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map) {
     umma::fence_after_sync();
     const uint32_t tmem = s_tmem, u_end = s_list.n_units;
     Waits waits;
-    auto wait_bar = [&](uint32_t b, uint32_t parity) {
-        waits.wait([&] {
-#pragma unroll 1
-            for (int i = 0; i < 64; ++i)
-                if (mbar_try_wait(b, parity)) return true;
-            return mbar_wait_timed(b, parity);
-        });
-    };
+    auto wait_bar = [&](uint32_t b, uint32_t parity) { waits.wait([&] { return wait_phase(b, parity); }); };
     auto entry = [&](const GroupUnit& g, uint32_t row) -> uint32_t { const uint32_t p = g.p0 + min(row, g.n - 1); return kGrouped ? a.pairs[p] : p; };
     auto tiles_of = [&](const GroupUnit& g) -> uint32_t { return (min(dg::kRows, a.M - g.m0) + 127) / 128; };
 
@@ -1218,19 +1189,18 @@ cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <int MODE, int NT>
+template <int MODE>
 cudaError_t group_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
-    using T = gg::Tile<NT>;
     constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
-    if (const cudaError_t e = allow_dynamic_smem<fp8_group_kernel<MODE, NT>>((int)T::kSmem)) return e;
-    if (const cudaError_t e = check_registers<fp8_group_kernel<MODE, NT>, gg::kRegLaunch>()) return e;
+    if (const cudaError_t e = allow_dynamic_smem<fp8_group_kernel<MODE>>((int)gg::kSmem)) return e;
+    if (const cudaError_t e = check_registers<fp8_group_kernel<MODE>, gg::kRegLaunch>()) return e;
     const uint64_t rows = (uint64_t)(kGrouped ? a.n_experts : 1u) * a.M;
     CUtensorMap m0, m1;
     if (rows > 0x7FFFFFFFu || !fp8_map(&m0, a.w[0], rows, a.K, 128) || !fp8_map(&m1, kGateUp ? a.w[1] : a.w[0], rows, a.K, 128)) return cudaErrorInvalidValue;
     // blocks: as many as there can be units
     const uint64_t per = kGateUp ? (a.M + 127) / 128 : (a.M + 255) / 256, pairs = kGrouped ? (uint64_t)a.n * a.n_used : a.n;
-    const uint64_t runs = kGrouped ? (pairs < a.n_experts ? pairs : pairs / NT + a.n_experts) : (pairs + NT - 1) / NT, units = per * runs;
-    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_group_kernel<MODE, NT>, dim3((uint32_t)(units < n_sms ? units : n_sms)), dim3(gg::kThreads), T::kSmem, a, m0, m1);
+    const uint64_t runs = kGrouped ? (pairs < a.n_experts ? pairs : pairs / gg::kNT + a.n_experts) : (pairs + gg::kNT - 1) / gg::kNT, units = per * runs;
+    const cudaError_t e = launch_kernel(Launch{L.stream, nullptr, true}, fp8_group_kernel<MODE>, dim3((uint32_t)(units < n_sms ? units : n_sms)), dim3(gg::kThreads), gg::kSmem, a, m0, m1);
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -1280,7 +1250,7 @@ template <int MODE>
 cudaError_t group_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
     const uint64_t mean = kGrouped ? (uint64_t)a.n * a.n_used / a.n_experts : a.n;
-    return mean > kManyPairs ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE, 32>(L, a, n_sms);
+    return mean > kManyPairs ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE>(L, a, n_sms);
 }
 
 // Which kernel a dense product takes: the least of these estimates, in us, fitted to measurements from 1 to 4096 rows, 1000 to 151,936 weight rows and K = 1040 to 4096.
@@ -1301,8 +1271,8 @@ cudaError_t dense_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     for (int i = 1; i < 5; ++i)
         if (wide[i] <= wide[best]) best = i;
     const double tiles = fmax(wide[best], read);
-    if (rows <= group && rows <= tiles) return launch_fp8_rows(L, kFp8Dense, a, n_sms);
-    if (group <= tiles) return group_launch<kFp8Dense, 32>(L, a, n_sms);
+    if (rows <= group && rows <= tiles) return launch_fp8_rows(L, kFp8Dense, a);
+    if (group <= tiles) return group_launch<kFp8Dense>(L, a, n_sms);
     switch (best) {
         case 0: return wide_launch<1, 32>(L, a, n_sms);
         case 1: return wide_launch<1, 64>(L, a, n_sms);
@@ -1323,7 +1293,7 @@ cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint
         case kFp8SharedGateUp: if (a.n > 64) return many_rows<kFp8SharedGateUp>(L, a, n_sms); break;
         case kFp8SharedDown: if (a.n > 64) return many_rows<kFp8SharedDown>(L, a, n_sms); break;
     }
-    return launch_fp8_rows(L, mode, a, n_sms);
+    return launch_fp8_rows(L, mode, a);
 }
 
 }  // namespace qkm

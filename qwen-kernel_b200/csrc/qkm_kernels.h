@@ -341,7 +341,7 @@ cudaError_t launch_argmax(const Launch& L, const float* logits, uint32_t n_rows,
 // ---- products with E4M3 weights (qkm_fp8.cu, qkm_fp8_gemm.cu; Fp8Args in qkm_fp8.cuh) ------------------------
 struct Fp8Args;
 cudaError_t launch_fp8_quantize(const Launch& L, const float* x, uint32_t n, uint32_t K, void* q, float* scale);
-cudaError_t launch_fp8_rows(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms);      // few rows
+cudaError_t launch_fp8_rows(const Launch& L, int mode, const Fp8Args& a);                      // few rows, dense or of the shared expert
 cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms);   // any number
 
 // ---- the router's balance loss and its gradient (qkm_balance.cu); scratch: balance_scratch_bytes(), zero before the first call
