@@ -200,6 +200,18 @@ fp8_rows_kernel(const Fp8Args a) {
     constexpr uint32_t kCols = 8 * NT;
     __shared__ float s_red[kRowsWarps * rows_mats<MODE>() * kCols * 16];
     pdl_trigger();
+    // The weights' lines come into the L2 while the kernel before ends (nothing is read yet: what that kernel may still write is seen by the loads).  With weights that are
+    // not there, quantiser and product in a graph: 1 x 8192 x 2048 8.3 -> 6.6 us, 1 x 4096 x 2048 5.8 -> 5.4.
+    if (blockIdx.y == 0) {
+        const uint32_t lane = threadIdx.x & 31u, row = blockIdx.x * 16u + (lane >> 1);
+        if (row < a.M)
+            for (uint32_t kb = threadIdx.x >> 5; kb < fp8_blocks(a.K); kb += kRowsWarps) {
+                const uint32_t c = kb * 128u + (lane & 1u) * 64u;
+                if (c < a.K)
+#pragma unroll
+                    for (int m = 0; m < rows_mats<MODE>(); ++m) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w[m] + (uint64_t)row * a.K + c));
+            }
+    }
     pdl_wait();
     for (uint32_t p = blockIdx.y * kCols; p < a.n; p += gridDim.y * kCols) rows_tile<MODE, NT, U>(a, blockIdx.x * 16u, p, s_red);
 }

@@ -82,7 +82,7 @@ def _check(got, want, T, E):
     assert np.all(np.abs(grad - w_grad) <= (E / 16 + 32) * 2.0**-24 * np.abs(size) + 1e-37)
 
 
-@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 256, 8), (3, 7, 2), (9, 60, 4), (64, 130, 6), (77, 512, 10), (500, 256, 8), (1000, 511, 16), (2500, 128, 8)])
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (1, 256, 8), (3, 7, 2), (9, 60, 4), (64, 130, 6), (77, 512, 10), (500, 256, 8), (1000, 511, 16), (2500, 128, 8), (20000, 256, 8)])
 @pytest.mark.parametrize("masked", [False, True])
 def test_balance(contexts, T, E, k, masked):
     rng = np.random.default_rng(T * 1000 + E)

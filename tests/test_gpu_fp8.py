@@ -78,7 +78,12 @@ SIZES = [(1, 1, 16), (1, 4096, 2048), (1, 257, 4096), (2, 130, 272), (5, 16, 128
          (1000, 512, 2048)]
 
 
-@pytest.mark.parametrize("n,M,K", SIZES)
+# every kind of tile, rows that fill no tile, results that start on no 16 bytes, one column block and odd numbers of them, several tiles a block
+TILES = [(16, 16400, 2048), (32, 50001, 272), (100, 4097, 2064), (250, 4100, 2048), (260, 4104, 1936), (64, 40001, 1040), (1000, 4100, 2048), (1030, 4101, 1040), (700, 20000, 128),
+         (2100, 9000, 272), (129, 30000, 400)]
+
+
+@pytest.mark.parametrize("n,M,K", SIZES + TILES)
 def test_gemm(ctx, n, M, K):
     rng = np.random.default_rng(n + 7 * M + 13 * K)
     w, ws = ref.weights(rng, M, K)
@@ -502,3 +507,50 @@ def test_layer_chain(pkg):
         assert np.all(np.abs(got - w * wd) <= w * bd + 2.0**-23 * np.abs(w * wd)), e
     fold = resid.astype(np.float64) + contrib.sum(1, dtype=np.float64) + y2
     assert np.all(np.abs(out - fold) <= (k + 3) * 2.0**-23 * (np.abs(resid) + np.abs(contrib).sum(1) + np.abs(y2)))
+
+
+def test_two_contexts_on_two_streams(pkg):
+    """Calls of two contexts under way at the same time give what they give one after the other."""
+    import torch
+    E, k, D, F, T = 16, 4, 1024, 512, 600
+    rng = np.random.default_rng(4)
+    dims = pkg.synth.Dims(n_embd=D, n_ff=F, n_expert=E, n_used=k)
+    sel, offsets, pairs = _selection(rng, T, E, k, 0.1)
+    mats = [t for shape in ((F, D), (F, D), (D, F)) for t in ref.weights(rng, *shape, mats=E)]
+    g, gs, u, us, d, ds, d_sel, d_off, d_pairs = [torch.from_numpy(np.ascontiguousarray(a).view(np.uint8).reshape(-1)).cuda() for a in (*mats, sel, offsets, pairs)]
+    logits = torch.randn((T, E), device="cuda")
+    runs = []
+    for i in range(2):
+        b = {"x": torch.randn((T, D), device="cuda"), "q": torch.empty((T, D), dtype=torch.uint8, device="cuda"), "s": torch.empty((T, D // 128), device="cuda"),
+             "h": torch.zeros((T, k + 1, F), device="cuda"), "hq": torch.empty((T * (k + 1), F), dtype=torch.uint8, device="cuda"),
+             "hs": torch.empty((T * (k + 1), F // 128), device="cuda"), "out": torch.zeros((T, k, D), device="cuda"), "y": torch.zeros((T, E * F), device="cuda"),
+             "counts": torch.zeros(E + 1, dtype=torch.int32, device="cuda"), "probs": torch.zeros(E, device="cuda"), "loss": torch.zeros(1, device="cuda")}
+        runs.append(b)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [pkg.Context(dims, n_layer=1, max_tokens=1, device=0) for _ in range(2)]
+
+    def step(c, b):
+        c.fp8_quantize(b["x"], T, D, b["q"], b["s"])
+        c.fp8_gemm(g, gs, b["q"], b["s"], b["y"], E * F, D, T)
+        c.moe_gateup_grouped_fp8(g, gs, u, us, b["q"], b["s"], d_off, d_pairs, b["h"], T)
+        c.fp8_quantize(b["h"], T * (k + 1), F, b["hq"], b["hs"])
+        c.moe_down_grouped_fp8(d, ds, b["hq"], b["hs"], d_sel, d_off, d_pairs, b["out"], T)
+        c.moe_balance(logits, d_sel, None, T, 1.0, b["counts"], b["probs"], b["loss"])
+
+    torch.cuda.synchronize()
+    want = []
+    for c, b, st in zip(ctxs, runs, streams):
+        c.set_stream(st.cuda_stream)
+        step(c, b)
+        c.sync()
+        want.append([b[n].clone() for n in ("y", "h", "out", "counts", "loss")])
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, b in zip(ctxs, runs):
+            step(c, b)
+    for c in ctxs:
+        c.sync()
+    for b, w in zip(runs, want):
+        assert all(torch.equal(b[n], t) for n, t in zip(("y", "h", "out", "counts", "loss"), w))
+    for c in ctxs:
+        c.close()
