@@ -4,6 +4,11 @@
 // tensor-memory columns of its own; eight warps read the set back, multiply it by the block's two scales and add it to the tile's f32 sums in registers,
 // while the MMAs of the next block run into another set.  Activation rows are the lanes (M), weight rows the columns (N): a thread holds one
 // row and a run of columns inside one block of 128 weight rows, so the scale is one number a thread and the scaling one FMA an element.
+//
+// What bounds it (4096 x 8192 x 4096 in tiles of 256 x 256, 122 us = 2.24 PFLOP/s; under the power cap, back to back, 154): the way out of tensor memory.  A block of 128 columns
+// is 514 cycles of MMA for a tile, but its 128 KB of sums take 340 cycles to read and 280 of FMAs (two elements each), which do not overlap much, and the hand-over of a set
+// either way some 100 each; with a tile's stores 900 in all.  1000 x 4096 x 2048: 12.6 us, of which 3.5 are the launch, 2 the stores.  Sixteen warps to scale and add took 138 us (the one that
+// issues MMAs waits behind 20 warps' polls), sets of 128 columns 139, an arrival with cluster scope 261 (a membar each).
 #include <cuda.h>
 
 #include <cmath>
@@ -349,6 +354,9 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
 // the gate and the up rows of one 128-row tile, or two tiles of one matrix, times a run; blocks take consecutive units, so that the runs of an expert
 // with more than 32 pairs read a tile from the L2.  Weight tiles come by TMA, the rows of the pairs with 16-byte copies, each row's scale of a
 // column block beside them; the eight warps that scale and add take the row scales from shared memory.
+//
+// What bounds it: memory, once it runs (gate/up of 16 tokens 32 us, 5.6 TB/s behind 5 us of start: the list of units, the first tiles; the 151,936 x 2048 head 55 us = 5.7 TB/s).  Up to 44 pairs an
+// expert it beats the kernels below (gate/up of 1024 tokens 113 us against 124, down 73 against 96); 64 columns a unit instead of 32 took 121 and 89.
 namespace gg {
 constexpr int kThreads = 512;                    // warps: 0 weights, 1 MMAs, 2 tensor memory, 4 - 7 rows, 8 - 15 scale and add
 constexpr int kRegAux = 40, kRegRows = 72, kRegAdd = 200;
@@ -723,7 +731,9 @@ __device__ __forceinline__ void put_columns(const float (&r)[16], uint32_t put, 
 // ---- the same with the pairs as lanes, for experts of many pairs ------------------------------------------------------------------------
 // A unit is up to 128 pairs (the MMAs' rows, a lane each) times 256 weight rows: the gate and the up rows of a 128-row tile, or two tiles of one matrix.  What a
 // thread scales is then one row's, as in the dense kernel: an FMA for two elements and nothing else.  (With the weight rows as lanes the scales of 128 columns came from shared
-// memory and the sums went out by single words: gate/up of 4096 tokens 281 us, down 243.)
+// memory and the sums went out by single words: gate/up of 4096 tokens 281 us, down 243.)  Now gate/up takes 176 us (196 to 215 back to back, under the power cap): 35 of them go
+// when nothing is scaled and added, 18 when no rows are copied, 13 when nothing is stored, 65 without all three - 565 MB from memory, 1.9 GB through the L2, tiles of 128 for 1.6 times the
+// pairs that there are.
 namespace pg {
 constexpr int kThreads = 512;                    // warps: 0 weights, 1 MMAs, 2 - 7 rows (2: tensor memory), 8 - 15 scale and add
 constexpr int kRowWarps = 6;
@@ -932,7 +942,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
 // ---- down products of many pairs and short sums ------------------------------------------------------------------------------------------
 // Of four column blocks or fewer a unit's results take as long to store as its sums to make.  Here a unit is 128 pairs times 512 weight rows, in tiles of 128: the pairs' rows stay in
 // shared memory for all of them, tiles come through a ring, and the two halves of the warps that scale and add take the tiles in turns, so that one stores while the other
-// adds.  (down of 4096 tokens, K = 512: the kernel above 174 us, 70 of them stores that nothing overlaps.)
+// adds.  (down of 4096 tokens, K = 512: the kernel above 174 us, 70 of them stores that nothing overlaps; this one 150, 45 of them stores.)
 namespace dg {
 constexpr uint32_t kMaxBlocks = 4, kRows = 512, kX = kMaxBlocks * 16384, kStages = 4, kSets = 4;
 constexpr uint32_t kW = 2 * kX, kPut = kW + kStages * 16384, kSmem = kPut + 8 * 2048 + 1024;   // x twice, weight tiles, 2 KB a warp on the way to coalesced stores
