@@ -244,6 +244,7 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
                 const float xc = x0, wc = w0;
                 if (kb + 1 < a.KB) { x0 = xs[kb + 1]; w0 = ws[kb + 1]; }
                 if (!ready) wait_bar(bar_set + 8 * set, parity);
+                __syncwarp();                                            // (each lane polls; the loads are the whole warp's)
                 umma::fence_after_sync();
                 const float s = xc * wc;
 #pragma unroll
@@ -344,6 +345,7 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
     umma::fence_before_sync();
     const int any_timed_out = __syncthreads_or(waits.out ? 1 : 0);
     if (any_timed_out) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies and MMAs still under way end long before this does
+    __syncwarp();
     if (CG == 2) cluster_sync();   // nothing of this block is read, written or signalled by the other one any more
     if (warp == 2) tmem_give_back<CG>(tmem);
     if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
@@ -695,6 +697,7 @@ fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     umma::fence_before_sync();
     const int any_timed_out = __syncthreads_or(waits.out ? 1 : 0);
     if (any_timed_out) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies and MMAs still under way end long before this does
+    __syncwarp();
     if (warp == 2) umma::tmem_dealloc(tmem, 512);
     if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
 }
@@ -804,6 +807,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
                 const float xc = x0, wac = wa0, wbc = wb0;
                 if (kb + 1 < KB) { x0 = xs[kb + 1]; wa0 = ws0[kb + 1]; wb0 = ws1[kb + 1]; }
                 if (!ready) wait_bar(bar_set + 8 * set, (blk >> 1) & 1u);
+                __syncwarp();                                // (each lane polls; the loads are the whole warp's)
                 umma::fence_after_sync();
                 float v[32];
                 if (work) {
@@ -935,6 +939,7 @@ fp8_pairs_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, cons
     umma::fence_before_sync();
     const int any_timed_out = __syncthreads_or(waits.out ? 1 : 0);
     if (any_timed_out) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies and MMAs still under way end long before this does
+    __syncwarp();
     if (warp == 2) umma::tmem_dealloc(tmem, 512);
     if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
 }
@@ -1015,6 +1020,7 @@ fp8_down_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map) {
                     if (kb >= KB) break;
                     const uint32_t set = (tile * KB + kb) % dg::kSets, t = t0 + set * 128u;
                     wait_bar(set0 + 8 * set, phases >> set & 1u);
+                    __syncwarp();                            // (each lane polls; the loads are the whole warp's)
                     phases ^= 1u << set;
                     umma::fence_after_sync();
                     const float s = x[kb] * w[kb];
@@ -1140,6 +1146,7 @@ fp8_down_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map) {
     umma::fence_before_sync();
     const int any_timed_out = __syncthreads_or(waits.out ? 1 : 0);
     if (any_timed_out) for (int i = 0; i < 100; ++i) __nanosleep(1000);   // copies and MMAs still under way end long before this does
+    __syncwarp();
     if (warp == 2) umma::tmem_dealloc(tmem, 512);
     if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
 }
