@@ -312,7 +312,8 @@ QKM_API int qkm_moe_shared_down_fp8(qkm_ctx *c, const void *down_shexp, const fl
  * N: tokens whose mask byte is not zero (mask NULL: all of them); counts[e]: how many of their selections (sel[t].ids[0..n_used), as
  * qkm_moe_select writes them; ids past the table are not counted) name expert e; probs[e]: the mean over these tokens of
  * softmax(logits[t])[e].  A logit that is not finite counts as -3.4e38, as in the selection.  counts: u32[n_expert + 1], the last one N;
- * probs f32[n_expert]; loss f32[1].  N = 0: all zero.  The result does not depend on the order in which blocks run.  n_tokens <= 2^24.
+ * probs f32[n_expert], to f32's rounding or 2^-62 * n_tokens, whichever is larger; loss f32[1].  N = 0: all zero.  The result does not
+ * depend on the order in which blocks run.  n_tokens <= 2^24.
  * (Sums in progress lie in the context: calls of one context on two streams must not overlap, nor replays of two graphs that captured them.) */
 QKM_API int qkm_moe_balance(qkm_ctx *c, const float *logits, const qkm_sel *sel, const uint8_t *mask,
                             uint32_t n_tokens, float coef, uint32_t *counts, float *probs, float *loss);

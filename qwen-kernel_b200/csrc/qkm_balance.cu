@@ -9,6 +9,7 @@
 //
 // What bounds it at 32768 x 256: the loss (14.9 us; 33.5 MB, 5.1 at the copy rate) waits for the sums over blocks, about 5 us of it, and issues some
 // 25 instructions an element; the gradient (14.7 us; 67 MB, 10.2) is near its traffic.
+#include <cmath>
 #include <type_traits>
 
 #include "qkm_common.cuh"
@@ -19,8 +20,14 @@ namespace {
 
 constexpr int kBalThreads = 256, kBalWarps = kBalThreads / 32;
 constexpr float kFloor = -3.4e38f;
-// Sums over blocks are added as integers of 2^-38: whatever their order, the result is the same.  n_tokens <= 2^24 keeps them inside 64 bits.
-constexpr double kFix = 274877906944.0;
+// Sums over blocks are added as integers of 1 / fix: whatever their order, the result is the same.  A sum is n_tokens at most, so fix is 2^62 over the power
+// of two that n_tokens does not pass: the sums stay inside 64 bits, and a mean is off by 2^-63 of that power at most (a rounding for each block that has a token
+// which counts): less than f32 rounds down to probabilities of 2^-39 where there is one token (2^-38 as fixed a unit lost those below 2^-15).
+double bal_fix(uint32_t n_tokens) {
+    int up = 0;
+    while (n_tokens > 1u << up) ++up;
+    return ldexp(1.0, 62 - up);
+}
 
 // what balance_kernel keeps between its blocks; all zero before and after a launch
 struct BalanceAcc {
@@ -92,7 +99,7 @@ __device__ __forceinline__ float row_exp(uint32_t E, uint32_t lane, float (&v)[V
 template <int V, bool VEC>
 __global__ void __launch_bounds__(kBalThreads)
 balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel, const uint8_t* __restrict__ mask, uint32_t n_tokens, uint32_t E, uint32_t n_used, float coef,
-               BalanceAcc* acc, uint32_t* __restrict__ counts, float* __restrict__ probs, float* __restrict__ loss) {
+               double fix, BalanceAcc* acc, uint32_t* __restrict__ counts, float* __restrict__ probs, float* __restrict__ loss) {
     __shared__ float s_p[kBalWarps][V * 32];
     __shared__ uint32_t s_cnt[V * 32];
     __shared__ uint32_t s_kept, s_last;
@@ -139,7 +146,7 @@ balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel
     for (uint32_t e = tid; e < E; e += kBalThreads) {
         double s = 0;
         for (int w = 0; w < kBalWarps; ++w) s += (double)s_p[w][e];
-        if (s != 0) atomicAdd(&acc->p[e], (unsigned long long)__double2ll_rn(s * kFix));
+        if (s != 0) atomicAdd(&acc->p[e], (unsigned long long)__double2ll_rn(s * fix));
         if (s_cnt[e]) atomicAdd(&acc->counts[e], s_cnt[e]);
     }
     if (tid == 0 && s_kept) atomicAdd(&acc->kept, s_kept);
@@ -153,7 +160,7 @@ balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel
     const double per = N ? 1.0 / N : 0.0;
     double sum = 0;
     for (uint32_t e = tid; e < E; e += kBalThreads) {
-        const double P = (double)__ldcg(&acc->p[e]) * (per / kFix);
+        const double P = (double)__ldcg(&acc->p[e]) * (per / fix);
         const uint32_t c = __ldcg(&acc->counts[e]);
         acc->p[e] = 0; acc->counts[e] = 0;
         counts[e] = c;
@@ -260,7 +267,7 @@ cudaError_t launch_balance(const Launch& L, const qkm_dims& d, const float* logi
                            uint32_t* counts, float* probs, float* loss, uint32_t n_sms) {
     const cudaError_t e = bal_variant(d.n_expert, d.n_expert % 4 == 0 && ((uintptr_t)logits & 15u) == 0, [&](auto v, auto vec) {
         return launch_kernel(Launch{L.stream, nullptr, true}, balance_kernel<v.value, vec.value>, dim3(bal_grid(n_tokens, n_sms, v.value <= 8 ? 4 : 3, bal_rows<v.value>())), dim3(kBalThreads), 0, logits, sel, mask,
-                             n_tokens, d.n_expert, d.n_used, coef, (BalanceAcc*)scratch, counts, probs, loss);
+                             n_tokens, d.n_expert, d.n_used, coef, bal_fix(n_tokens), (BalanceAcc*)scratch, counts, probs, loss);
     });
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();

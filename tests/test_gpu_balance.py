@@ -162,3 +162,20 @@ def test_balance_of_nothing_and_refusals(contexts, pkg):
         assert ei.value.code == code
     for b in (d, d_counts, d_probs, d_loss):
         b.free()
+
+
+@pytest.mark.parametrize("T,E,k,kept", [(1, 64, 4, 1), (1, 512, 10, 1), (3, 60, 4, 2), (40, 256, 8, 3), (3000, 128, 8, 5)])
+def test_small_probabilities_of_few_tokens(contexts, T, E, k, kept):
+    """Probabilities down to e^-24 of the largest; logits are multiples of 2^-10, so their distances from the largest are exact.  Of itself a mean carries what _check counts, and beside that 2^-63 of the power of two above T (the
+    rounding of its sum, an integer of 2^-62 of that power, once for each block that has a token, so at most once a token)."""
+    rng = np.random.default_rng(T + E)
+    logits = (np.round(rng.uniform(-24, 0, (T, E)) * 1024) / 1024).astype(np.float32)
+    sel = _records(rng, T, E, k)
+    mask = np.zeros(T, np.uint8)
+    mask[rng.permutation(T)[:kept]] = 1
+    counts, probs, loss, _ = _run(contexts(E, k), logits, sel, mask, 1.0, None)
+    w_counts, N, w_probs, w_loss, _, _ = _reference(logits, sel["ids"][:, :k], mask, 1.0, 1.0)
+    assert N == kept and counts[E] == kept and np.array_equal(counts[:E], w_counts)
+    rel, least = (E / 32 + 12 + min(kept, 64)) * 2.0**-24, 2.0**-63 * 2 ** int(np.ceil(np.log2(T)))
+    assert np.all(np.abs(probs - w_probs) <= rel * w_probs + least), np.max(np.abs(probs - w_probs) / w_probs)
+    assert abs(loss - w_loss) <= rel * w_loss + least * E
