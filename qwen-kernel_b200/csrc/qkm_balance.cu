@@ -221,7 +221,9 @@ balance_grad_kernel(const float* logits, const uint8_t* __restrict__ mask, const
                 dot = warp_sum(dot);
 #pragma unroll
                 for (int i = 0; i < V; ++i) v[r][i] *= g[i] - dot;
-                if (low)                           // logits at the floor count here: those that are not finite get no gradient
+                // Logits that are not finite get no gradient.  Where every logit is at the floor they count; where some g is not finite (then the row's mean is not
+                // either) their zero probability does not make them zero.
+                if (low || !isfinite(dot))
 #pragma unroll 1
                     for (int i = 0; i < V; ++i)
                         if (bal_col<VEC>(lane, i) < E && !isfinite(logits[(size_t)t * E + bal_col<VEC>(lane, i)])) drop(v[r], i);

@@ -179,3 +179,21 @@ def test_small_probabilities_of_few_tokens(contexts, T, E, k, kept):
     rel, least = (E / 32 + 12 + min(kept, 64)) * 2.0**-24, 2.0**-63 * 2 ** int(np.ceil(np.log2(T)))
     assert np.all(np.abs(probs - w_probs) <= rel * w_probs + least), np.max(np.abs(probs - w_probs) / w_probs)
     assert abs(loss - w_loss) <= rel * w_loss + least * E
+
+
+@pytest.mark.parametrize("E,k", [(64, 4), (61, 3), (300, 8)])
+@pytest.mark.parametrize("upstream", [np.inf, -np.inf, np.nan, 3e38])
+def test_gradient_where_the_upstream_is_not_finite(contexts, E, k, upstream):
+    """A loss scale that overflowed: tokens that the mask leaves out and logits that are not finite get zero all the same, the rest nothing
+    finite.  (3e38 times a coefficient of 100 passes f32 too.)"""
+    T = 20
+    rng = np.random.default_rng(E)
+    logits = rng.standard_normal((T, E)).astype(np.float32)
+    logits[0, 5:20], logits[1, 3], logits[2, 4], logits[3, :], logits[4, :E - 1] = -np.inf, np.nan, np.inf, -np.inf, np.nan
+    sel = _records(rng, T, E, k)
+    sel["ids"][:, 0], sel["ids"][:, 1:k] = 7, 9
+    mask = np.ones(T, np.uint8)
+    mask[10:14] = 0
+    grad = _run(contexts(E, k), logits, sel, mask, 100.0, upstream)[3]
+    zero = ~np.isfinite(logits) | (mask == 0)[:, None]
+    assert np.all(grad[zero] == 0) and not np.isfinite(grad[~zero]).any()
