@@ -314,7 +314,8 @@ QKM_API int qkm_moe_shared_down_fp8(qkm_ctx *c, const void *down_shexp, const fl
  * softmax(logits[t])[e].  A logit that is not finite counts as -3.4e38, as in the selection.  counts: u32[n_expert + 1], the last one N;
  * probs f32[n_expert], to f32's rounding or 2^-62 * n_tokens, whichever is larger; loss f32[1].  N = 0: all zero.  The result does not
  * depend on the order in which blocks run.  n_tokens <= 2^24.
- * (Sums in progress lie in the context: calls of one context on two streams must not overlap, nor replays of two graphs that captured them.) */
+ * (Sums in progress lie in the context: calls of one context on two streams must not overlap, nor replays of two graphs that captured them;
+ * where they do, each may get the other's sums.  Calls after them are not touched.) */
 QKM_API int qkm_moe_balance(qkm_ctx *c, const float *logits, const qkm_sel *sel, const uint8_t *mask,
                             uint32_t n_tokens, float coef, uint32_t *counts, float *probs, float *loss);
 /* d_logits[t][e] = d loss / d logits[t][e] times *d_loss (device f32; NULL: 1), from the counts of qkm_moe_balance (or their sums over

@@ -7,8 +7,8 @@
 // (shaders/moe_select.comp:28-34), and gets none.  A warp holds a row in registers, the same columns in the same lane for every row, so a lane adds up its
 // columns' probabilities - and keeps its columns' g - in registers.
 //
-// What bounds it at 32768 x 256: the loss (14.9 us; 33.5 MB, 5.1 at the copy rate) waits for the sums over blocks, about 5 us of it, and issues some
-// 25 instructions an element; the gradient (14.7 us; 67 MB, 10.2) is near its traffic.
+// What bounds it at 32768 x 256: the loss (14.9 us; 33.5 MB, 5.1 at the copy rate) issues some 25 instructions an element, and ends with additions of all blocks to
+// the same sums and a kernel that reads them; the gradient (14.4 us; 67 MB, 10.2) is near its traffic.
 #include <cmath>
 #include <type_traits>
 
@@ -29,11 +29,13 @@ double bal_fix(uint32_t n_tokens) {
     return ldexp(1.0, 62 - up);
 }
 
-// what balance_kernel keeps between its blocks; all zero before and after a launch
+// Sums of balance_kernel, which balance_finish_kernel reads and sets back to zero.  Calls of two streams that overlap add to the same sums and get wrong
+// results; but whichever of their finish kernels runs last has every addition before it and leaves zeros, so that nothing of them reaches a later call.
+// (With the last block of one kernel, told by a count, in place of the second kernel, the count and the sums could stay wrong for good.)
 struct BalanceAcc {
     unsigned long long p[512];
     uint32_t counts[512];
-    uint32_t kept, ticket;
+    uint32_t kept;
 };
 
 // V values a lane: column of value i
@@ -96,14 +98,14 @@ __device__ __forceinline__ float row_exp(uint32_t E, uint32_t lane, float (&v)[V
     return __fdividef(1.f, warp_sum(sum));     // (1 <= sum <= 512)
 }
 
+// (8 values a lane: without the number of blocks (0: none given) the compiler takes 48 registers and one row's loads at a time, 16.8 us of 32768 x 256 instead of 14.9)
 template <int V, bool VEC>
-__global__ void __launch_bounds__(kBalThreads)
-balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel, const uint8_t* __restrict__ mask, uint32_t n_tokens, uint32_t E, uint32_t n_used, float coef,
-               double fix, BalanceAcc* acc, uint32_t* __restrict__ counts, float* __restrict__ probs, float* __restrict__ loss) {
+__global__ void __launch_bounds__(kBalThreads, V == 8 ? 4 : 0)
+balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel, const uint8_t* __restrict__ mask, uint32_t n_tokens, uint32_t E, uint32_t n_used, double fix,
+               BalanceAcc* acc) {
     __shared__ float s_p[kBalWarps][V * 32];
     __shared__ uint32_t s_cnt[V * 32];
-    __shared__ uint32_t s_kept, s_last;
-    __shared__ double s_sum[kBalWarps];
+    __shared__ uint32_t s_kept;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     for (uint32_t i = tid; i < V * 32; i += kBalThreads) s_cnt[i] = 0;
     if (tid == 0) s_kept = 0;
@@ -150,31 +152,36 @@ balance_kernel(const float* __restrict__ logits, const qkm_sel* __restrict__ sel
         if (s_cnt[e]) atomicAdd(&acc->counts[e], s_cnt[e]);
     }
     if (tid == 0 && s_kept) atomicAdd(&acc->kept, s_kept);
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) s_last = atomicAdd(&acc->ticket, 1u) == gridDim.x - 1 ? 1u : 0u;
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
-    const uint32_t N = __ldcg(&acc->kept);
+}
+
+// One block, a thread an expert; unit: 1 / fix, factor: coef * E / n_used
+constexpr int kFinThreads = 512;
+__global__ void __launch_bounds__(kFinThreads)
+balance_finish_kernel(BalanceAcc* acc, uint32_t E, double unit, double factor, uint32_t* __restrict__ counts, float* __restrict__ probs, float* __restrict__ loss) {
+    __shared__ double s_sum[kFinThreads / 32];
+    const uint32_t e = threadIdx.x;
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t N = acc->kept;
     const double per = N ? 1.0 / N : 0.0;
     double sum = 0;
-    for (uint32_t e = tid; e < E; e += kBalThreads) {
-        const double P = (double)__ldcg(&acc->p[e]) * (per / fix);
-        const uint32_t c = __ldcg(&acc->counts[e]);
+    if (e < E) {
+        const uint32_t c = acc->counts[e];
+        const double P = (double)acc->p[e] * unit * per;
         acc->p[e] = 0; acc->counts[e] = 0;
         counts[e] = c;
         probs[e] = (float)P;
-        sum += (double)c * P;
+        sum = (double)c * P;
     }
     sum = warp_sum(sum);
-    if (lane == 0) s_sum[warp] = sum;
+    if ((e & 31u) == 0) s_sum[e >> 5] = sum;
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kBalWarps; ++w) sum += s_sum[w];
+    if (e >= 32) return;
+    sum = warp_sum(e < kFinThreads / 32 ? s_sum[e] : 0.0);
+    if (e == 0) {
         counts[E] = N;
-        *loss = (float)(sum * per * ((double)coef * E / n_used));
-        acc->kept = 0; acc->ticket = 0;
+        *loss = (float)(sum * per * factor);
+        acc->kept = 0;
     }
 }
 
@@ -187,13 +194,13 @@ __device__ __forceinline__ void drop(float (&v)[V], int at) {
 
 template <int V, bool VEC>
 __global__ void __launch_bounds__(kBalThreads)
-balance_grad_kernel(const float* logits, const uint8_t* __restrict__ mask, const uint32_t* __restrict__ counts, uint32_t n_tokens, uint32_t E, uint32_t n_used, float coef,
+balance_grad_kernel(const float* logits, const uint8_t* __restrict__ mask, const uint32_t* __restrict__ counts, uint32_t n_tokens, uint32_t E, double factor,
                     const float* __restrict__ d_loss, float* d_logits) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     pdl_trigger();
     pdl_wait();
     const uint32_t N = counts[E];
-    const double unit = N ? (double)coef * E / n_used / N / N * (d_loss ? (double)*d_loss : 1.0) : 0.0;
+    const double up = d_loss ? (double)*d_loss : 1.0, unit = N ? factor / ((double)N * N) * up : 0.0;
     float g[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) g[i] = bal_col<VEC>(lane, i) < E ? (float)(unit * counts[bal_col<VEC>(lane, i)]) : 0.f;
@@ -267,10 +274,18 @@ size_t balance_scratch_bytes() { return sizeof(BalanceAcc); }
 
 cudaError_t launch_balance(const Launch& L, const qkm_dims& d, const float* logits, const qkm_sel* sel, const uint8_t* mask, uint32_t n_tokens, float coef, void* scratch,
                            uint32_t* counts, float* probs, float* loss, uint32_t n_sms) {
-    const cudaError_t e = bal_variant(d.n_expert, d.n_expert % 4 == 0 && ((uintptr_t)logits & 15u) == 0, [&](auto v, auto vec) {
-        return launch_kernel(Launch{L.stream, nullptr, true}, balance_kernel<v.value, vec.value>, dim3(bal_grid(n_tokens, n_sms, v.value <= 8 ? 4 : 3, bal_rows<v.value>())), dim3(kBalThreads), 0, logits, sel, mask,
-                             n_tokens, d.n_expert, d.n_used, coef, bal_fix(n_tokens), (BalanceAcc*)scratch, counts, probs, loss);
-    });
+    const Launch P{L.stream, nullptr, true};
+    const double fix = bal_fix(n_tokens);
+    cudaError_t e = cudaSuccess;
+    if (n_tokens) {
+        e = bal_variant(d.n_expert, d.n_expert % 4 == 0 && ((uintptr_t)logits & 15u) == 0, [&](auto v, auto vec) {
+            return launch_kernel(P, balance_kernel<v.value, vec.value>, dim3(bal_grid(n_tokens, n_sms, v.value <= 8 ? 4 : 3, bal_rows<v.value>())), dim3(kBalThreads), 0, logits, sel, mask,
+                                 n_tokens, d.n_expert, d.n_used, fix, (BalanceAcc*)scratch);
+        });
+        L.count();
+        if (e != cudaSuccess) return e;
+    }
+    e = launch_kernel(P, balance_finish_kernel, dim3(1), dim3(kFinThreads), 0, (BalanceAcc*)scratch, d.n_expert, 1.0 / fix, (double)coef * d.n_expert / d.n_used, counts, probs, loss);
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();
 }
@@ -281,7 +296,7 @@ cudaError_t launch_balance_grad(const Launch& L, const qkm_dims& d, const float*
     const bool vec = d.n_expert % 4 == 0 && (((uintptr_t)logits | (uintptr_t)d_logits) & 15u) == 0;
     const cudaError_t e = bal_variant(d.n_expert, vec, [&](auto v, auto ve) {
         return launch_kernel(Launch{L.stream, nullptr, true}, balance_grad_kernel<v.value, ve.value>, dim3(bal_grid(n_tokens, n_sms, v.value == 8 ? 6 : 4, bal_rows<v.value>())), dim3(kBalThreads), 0, logits, mask,
-                             counts, n_tokens, d.n_expert, d.n_used, coef, d_loss, d_logits);
+                             counts, n_tokens, d.n_expert, (double)coef * d.n_expert / d.n_used, d_loss, d_logits);
     });
     L.count();
     return e != cudaSuccess ? e : cudaGetLastError();

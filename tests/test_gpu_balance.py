@@ -197,3 +197,28 @@ def test_gradient_where_the_upstream_is_not_finite(contexts, E, k, upstream):
     grad = _run(contexts(E, k), logits, sel, mask, 100.0, upstream)[3]
     zero = ~np.isfinite(logits) | (mask == 0)[:, None]
     assert np.all(grad[zero] == 0) and not np.isfinite(grad[~zero]).any()
+
+
+def test_calls_that_overlapped_leave_nothing_behind(contexts):
+    """Two streams' calls of one context at the same time get each other's sums, as the header says; the calls after them do not."""
+    import torch
+    E, k = 256, 8
+    c = contexts(E, k)
+    rng = np.random.default_rng(1)
+    parts = []
+    for T in (2000, 700):
+        logits, sel = rng.standard_normal((T, E)).astype(np.float32), _records(rng, T, E, k)
+        parts.append((T, logits, sel, torch.from_numpy(logits).cuda(), torch.from_numpy(sel.view(np.uint8).reshape(T, -1)).cuda(),
+                      torch.zeros(E + 1, dtype=torch.int32, device="cuda"), torch.zeros(E, device="cuda"), torch.zeros(1, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    try:
+        for _ in range(200):
+            for T, _, _, d_logits, d_sel, counts, probs, loss, st in parts:
+                c.set_stream(st.cuda_stream)
+                c.moe_balance(d_logits, d_sel, None, T, 0.01, counts, probs, loss)
+        torch.cuda.synchronize()
+    finally:
+        c.set_stream(0)
+    for _ in range(2):
+        for T, logits, sel, *_ in parts:
+            _check(_run(c, logits, sel, None, 0.01, 1.5), _reference(logits, sel["ids"][:, :k], None, 0.01, 1.5), T, E)
