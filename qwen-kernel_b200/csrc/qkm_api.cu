@@ -1140,7 +1140,7 @@ int fp8_product(qkm_ctx* c, const char* name, int mode, const void* w0, const fl
     Fp8Args a{};
     a.w[0] = (const uint8_t*)w0; a.w[1] = (const uint8_t*)w1; a.w_scale[0] = s0; a.w_scale[1] = s1;
     a.xq = (const uint8_t*)xq; a.x_scale = xs; a.offsets = offsets; a.pairs = pairs; a.sel = sel; a.out = out;
-    a.M = M; a.K = K; a.n = n; a.n_experts = c->ecount; a.n_used = c->cfg.dims.n_used; a.status = c->status;
+    a.M = M; a.K = K; a.n = n; a.n_experts = c->ecount; a.n_table = c->cfg.dims.n_expert; a.n_used = c->cfg.dims.n_used; a.status = c->status;
     QKM_LAUNCH(c, launch_fp8_product(c->L(), mode, a, (uint32_t)c->n_sms));
     return QKM_OK;
 }

@@ -23,7 +23,8 @@ struct Fp8Args {
     const qkm_sel* sel;            // routing weights of the down products
     float* out;
     uint32_t M, K, n;              // n: rows (dense), tokens otherwise
-    uint32_t n_experts, n_used;
+    uint32_t n_experts, n_used;    // experts of w and offsets
+    uint32_t n_table;              // experts of the whole table, of which these may be a shard
     uint32_t* status;
 };
 

@@ -15,6 +15,7 @@
 
 #include "qkm_common.cuh"
 #include "qkm_fp8.cuh"
+#include "qkm_fp8_choice.h"
 #include "qkm_umma.cuh"
 #include "qkm_wait.h"
 
@@ -1260,14 +1261,9 @@ cudaError_t many_rows(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     return pairs_launch<MODE>(L, a, n_sms);
 }
 
-// Pairs an expert, on average, from which they are the lanes: gate/up of 2048 tokens (64) 162 us as columns, 135 as lanes, of 1024 113 and 124; down 112, 108 and 73, 96.
-constexpr uint64_t kManyPairs = 44;
-
 template <int MODE>
 cudaError_t group_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
-    constexpr bool kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
-    const uint64_t mean = kGrouped ? (uint64_t)a.n * a.n_used / a.n_experts : a.n;
-    return mean > kManyPairs ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE>(L, a, n_sms);
+    return fp8_pairs_as_lanes(a.n, a.n_used, a.n_table) ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE>(L, a, n_sms);
 }
 
 // Which kernel a dense product takes: the least of these estimates, in us, fitted to measurements from 1 to 4096 rows, 1000 to 151,936 weight rows and K = 1040 to 4096.
