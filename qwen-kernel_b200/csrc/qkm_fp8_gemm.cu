@@ -1263,7 +1263,7 @@ cudaError_t many_rows(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
 
 template <int MODE>
 cudaError_t group_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
-    return fp8_pairs_as_lanes(a.n, a.n_used, a.n_table) ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE>(L, a, n_sms);
+    return fp8_pairs_as_lanes(MODE == kFp8Down, a.n, a.n_used, a.n_table) ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE>(L, a, n_sms);
 }
 
 // Which kernel a dense product takes: the least of these estimates, in us, fitted to measurements from 1 to 4096 rows, 1000 to 151,936 weight rows and K = 1040 to 4096.
@@ -1303,8 +1303,8 @@ cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint
         case kFp8Dense: return dense_any(L, a, n_sms);
         case kFp8GateUp: return group_any<kFp8GateUp>(L, a, n_sms);
         case kFp8Down: return group_any<kFp8Down>(L, a, n_sms);
-        case kFp8SharedGateUp: if (a.n > 64) return many_rows<kFp8SharedGateUp>(L, a, n_sms); break;
-        case kFp8SharedDown: if (a.n > 64) return many_rows<kFp8SharedDown>(L, a, n_sms); break;
+        case kFp8SharedGateUp: if (!fp8_shared_few_rows(false, a.n, a.M, a.K)) return many_rows<kFp8SharedGateUp>(L, a, n_sms); break;
+        case kFp8SharedDown: if (!fp8_shared_few_rows(true, a.n, a.M, a.K)) return many_rows<kFp8SharedDown>(L, a, n_sms); break;
     }
     return launch_fp8_rows(L, mode, a);
 }
