@@ -11,8 +11,6 @@
 // issues MMAs waits behind 20 warps' polls), sets of 128 columns 139, an arrival with cluster scope 261 (a membar each).
 #include <cuda.h>
 
-#include <cmath>
-
 #include "qkm_common.cuh"
 #include "qkm_fp8.cuh"
 #include "qkm_fp8_choice.h"
@@ -1266,40 +1264,24 @@ cudaError_t group_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
     return fp8_pairs_as_lanes(MODE == kFp8Down, a.n, a.n_used, a.n_table) ? many_rows<MODE>(L, a, n_sms) : group_launch<MODE>(L, a, n_sms);
 }
 
-// Which kernel a dense product takes: the least of these estimates, in us, fitted to measurements from 1 to 4096 rows, 1000 to 151,936 weight rows and K = 1040 to 4096.
-// Tiles go over the machine in waves whose length is that of a tile (at K = 2048: 5.0 us for 128 x 32, 5.5 for 128 x 64, 8.5 for 128 x 256; of pairs of blocks 6.2 for
-// 256 x 128, 8.5 for 256 x 256), so that few rows or a small matrix want small tiles and large ones those that read least.  Of at most 32 rows the weights are what is
-// read: by warps straight from memory where the matrix is small (16 x 4096 x 2048 5.2 us, group tiles 9.8, 128 x 32 8.4), through the group kernel's ring where it is large
-// (1 x 151,936 x 2048 55 us against 60 and 65; 16 rows 57 against 111 and 59).
 cudaError_t dense_any(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
-    const double mb = (double)a.M * a.K * 1e-6, k = a.K / 2048.0;
-    auto waves = [&](uint32_t rows, uint32_t cols, uint32_t slots) {
-        const uint64_t tiles = (uint64_t)((a.n + rows - 1) / rows) * ((a.M + cols - 1) / cols);
-        return (double)((tiles + slots - 1) / slots) * k;
-    };
-    const double rows = (a.n <= 8 ? 0.19 : 0.3 * ((a.n + 15) / 16)) * mb - 0.5;
-    const double group = a.n > 32 ? 1e30 : fmax(6.3 * waves(32, 256, n_sms), mb / 5.9), read = mb / 4.9;
-    const double wide[5] = {5.0 * waves(128, 32, n_sms), 5.5 * waves(128, 64, n_sms), 6.2 * waves(256, 128, n_sms / 2), 8.5 * waves(128, 256, n_sms), 8.5 * waves(256, 256, n_sms / 2)};
-    int best = 0;
-    for (int i = 1; i < 5; ++i)
-        if (wide[i] <= wide[best]) best = i;
-    const double tiles = fmax(wide[best], read);
-    if (rows <= group && rows <= tiles) return launch_fp8_rows(L, kFp8Dense, a);
-    if (group <= tiles) return group_launch<kFp8Dense>(L, a, n_sms);
-    switch (best) {
-        case 0: return wide_launch<1, 32>(L, a, n_sms);
-        case 1: return wide_launch<1, 64>(L, a, n_sms);
-        case 2: return wide_launch<2, 128>(L, a, n_sms);
-        case 3: return wide_launch<1, 256>(L, a, n_sms);
-        default: return wide_launch<2, 256>(L, a, n_sms);
+    switch (fp8_dense_kernel(a.n, a.M, a.K, n_sms)) {
+        case Fp8Dense::kRows: return launch_fp8_rows(L, kFp8Dense, a);
+        case Fp8Dense::kGroup: return group_launch<kFp8Dense>(L, a, n_sms);
+        case Fp8Dense::k128x32: return wide_launch<1, 32>(L, a, n_sms);
+        case Fp8Dense::k128x64: return wide_launch<1, 64>(L, a, n_sms);
+        case Fp8Dense::k256x128: return wide_launch<2, 128>(L, a, n_sms);
+        case Fp8Dense::k128x256: return wide_launch<1, 256>(L, a, n_sms);
+        case Fp8Dense::k256x256: return wide_launch<2, 256>(L, a, n_sms);
     }
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
 cudaError_t launch_fp8_product(const Launch& L, int mode, const Fp8Args& a, uint32_t n_sms) {
     if (a.n == 0 || a.M == 0) return cudaSuccess;
-    if (a.K >= 128) switch (mode) {
+    switch (mode) {
         case kFp8Dense: return dense_any(L, a, n_sms);
         case kFp8GateUp: return group_any<kFp8GateUp>(L, a, n_sms);
         case kFp8Down: return group_any<kFp8Down>(L, a, n_sms);

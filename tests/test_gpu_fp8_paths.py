@@ -39,3 +39,158 @@ def test_shared_expert_with_rows_as_lanes(pkg, D, F, T):
             wd, bd = ref.product(d, ds, hq[at], hs[at])
             w = sel["w_shared"].astype(np.float64)[:, None]
             assert np.all(np.abs(y2 - w * wd) <= w * bd + 2.0**-23 * np.abs(w * wd))
+
+
+# rows, weight rows and columns that take each kernel; no size fills a tile, the last column block is short
+PATHS = {"rows": (40, 300, 400), "group": (16, 20003, 400), "128x32": (200, 1010, 400), "128x64": (260, 2110, 400), "256x128": (300, 4110, 400), "128x256": (100, 20003, 400),
+         "256x256": (520, 4110, 400)}
+assert set(PATHS) == set(choice.DENSE)
+
+
+@pytest.fixture(scope="module")
+def ctx(pkg):
+    c = pkg.Context(pkg.synth.Dims(), n_layer=1, max_tokens=16, device=0)
+    yield c
+    c.close()
+
+
+@pytest.fixture(scope="module")
+def n_sms():
+    import torch
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+def _gemm(ctx, w, ws, q, s):
+    M, (n, K) = w.shape[0], q.shape
+    d = _dev(ctx, w, ws, q, s)
+    d_y, = _dev(ctx, np.full(n * M + 64, -7.25, np.float32))
+    ctx.fp8_gemm(*d, d_y, M, K, n)
+    ctx.sync()
+    y = d_y.download(np.float32, n * M + 64)
+    _free(*d, d_y)
+    assert np.all(y[n * M:] == -7.25)
+    return y[:n * M].reshape(n, M)
+
+
+def _by_blocks(w, ws, q, s):
+    """(y, bound, sure): the definition with every block's sum scaled as a whole, so that a scale may be infinite; how far finite results may be off (fp8_ref.product);
+    whether an infinite one's sign is beyond rounding."""
+    W, X = ref.decode(w), ref.decode(q)
+    (M, K), n = W.shape, X.shape[0]
+    y, size, sure = np.zeros((n, M)), np.zeros((n, M)), np.ones((n, M), bool)
+    with np.errstate(invalid="ignore", over="ignore"):
+        for b in range(ref.blocks(K)):
+            at = slice(128 * b, min(128 * b + 128, K))
+            scale = s[:, b].astype(np.float64)[:, None] * ws[:, b].astype(np.float64).repeat(128)[:M]
+            sums, sizes = X[:, at] @ W[:, at].T, np.abs(X[:, at]) @ np.abs(W[:, at]).T
+            y += scale * sums
+            size += np.abs(scale) * sizes
+            sure &= ~np.isinf(scale) | (np.abs(sums) > sizes * 2.0**-16)
+    return y, size * 2.0**-23 * (128 + ref.blocks(K) + 4), sure
+
+
+def _same(got, want, bound, sure):
+    infinite = np.isinf(want)
+    assert sure.mean() > 0.99
+    assert np.array_equal(np.isnan(got)[sure], np.isnan(want)[sure])
+    assert np.array_equal(got[infinite & sure], want[infinite & sure])
+    there = np.isfinite(want)
+    off = np.abs(got[there] - want[there])
+    assert np.all(off <= bound[there]), np.max(off / bound[there])
+
+
+@pytest.mark.parametrize("path", choice.DENSE)
+def test_a_spoilt_row_spoils_itself_alone(ctx, n_sms, path):
+    """NaN codes in the first, a middle and the last row of either side, in the first column, a middle one and the last of the short block; scales of zero, negative and infinite
+    ones.  Rows and columns of a tile that are not there, and what an earlier tile left in shared memory, reach nothing."""
+    n, M, K = PATHS[path]
+    assert choice.dense_kernel(n, M, K, n_sms) == path
+    rng = np.random.default_rng(n)
+    w, ws = ref.weights(rng, M, K)
+    q, s = ref.quantize(rng.standard_normal((n, K)).astype(np.float32))
+    spoilt = w.copy(), q.copy()
+    for row, col in ((0, K - 1), (M // 2, 130), (M - 1, 0)):
+        spoilt[0][row, col] = 127
+    for row, col in ((0, 0), (n // 2, K - 1), (n - 1, 255)):
+        spoilt[1][row, col] = 255
+    ws[0, 1], s[n - 2, 2], ws[1, 0] = 0, 0, -0.01
+    _same(_gemm(ctx, spoilt[0], ws, spoilt[1], s), *_by_blocks(spoilt[0], ws, spoilt[1], s))
+    s[3, 0], ws[M // 256, 2] = np.inf, -np.inf
+    _same(_gemm(ctx, w, ws, q, s), *_by_blocks(w, ws, q, s))
+
+
+@pytest.mark.parametrize("path", choice.DENSE)
+def test_small_products_beside_a_large_one(ctx, n_sms, path):
+    """A block's sum keeps what is 2^-23 of it: 2^-9 in every column but one of 448 times 1 and 448, at the block's start, inside it and at its end."""
+    n, M, K = PATHS[path]
+    assert choice.dense_kernel(n, M, K, n_sms) == path
+    w = np.full((M, K), ref.encode(1.0), np.uint8)
+    q = np.full((n, K), 1, np.uint8)
+    for b, at in enumerate((0, 128 + 77, 256 + 127, K - 1)):
+        q[:, at] = 126 if b % 2 else 254
+        w[1::2, at] = 126
+    ones = np.ones((ref.blocks(M), ref.blocks(K)), np.float32), np.ones((n, ref.blocks(K)), np.float32)
+    _same(_gemm(ctx, w, ones[0], q, ones[1]), *_by_blocks(w, ones[0], q, ones[1]))
+
+
+@pytest.mark.parametrize("path", choice.DENSE)
+def test_blocks_that_cancel(ctx, n_sms, path):
+    """Two blocks 2^30 above the others, one the other's opposite: what f32 sums keep of the rest stays."""
+    n, M, K = PATHS[path]
+    assert choice.dense_kernel(n, M, K, n_sms) == path
+    rng = np.random.default_rng(M)
+    w, ws = ref.weights(rng, M, K)
+    q, s = ref.quantize(rng.standard_normal((n, K)).astype(np.float32))
+    w[:, 128:256] = w[:, :128]
+    q[:, 128:256] = q[:, :128] ^ 128
+    s[:, 1] = s[:, 0]
+    ws[:, 0] = ws[:, 1] = 2.0**20
+    _same(_gemm(ctx, w, ws, q, s), *_by_blocks(w, ws, q, s))
+
+
+# tokens, experts, selections, hidden, inner: gate/up and down by columns, by lanes (down of few column blocks and of more)
+EXPERT_PATHS = [(20, 4, 2, 256, 256), (300, 4, 2, 512, 256), (300, 4, 2, 256, 768)]
+
+
+@pytest.mark.parametrize("T,E,k,D,F", EXPERT_PATHS)
+def test_a_spoilt_pair_spoils_itself_alone(pkg, T, E, k, D, F):
+    """NaN codes in one weight row of an expert and in single tokens' rows, zero, negative and infinite scales, a large product beside small ones: every other result of
+    gate/up and down is as without them."""
+    lanes = T == 300
+    assert choice.pairs_as_lanes(False, T, k, E) == choice.pairs_as_lanes(True, T, k, E) == lanes
+    rng = np.random.default_rng(T + F)
+    dims = pkg.synth.Dims(n_embd=D, n_ff=F, n_expert=E, n_used=k)
+    sel, offsets, pairs = _selection(rng, T, E, k)
+    q, s = ref.quantize(rng.standard_normal((T, D)).astype(np.float32))
+    hq, hs = ref.quantize(rng.standard_normal((T * (k + 1), F)).astype(np.float32))
+    (g, gs), (u, us), (d, ds) = (ref.weights(rng, *shape, mats=E) for shape in ((F, D), (F, D), (D, F)))
+    g[1, 0, D - 1], u[2, F - 1, 0], d[1, D // 2, 130], d[3, D - 1, F - 1] = 127, 255, 127, 255
+    q[T - 1, D - 1], hq[0, 0], hq[(T // 2) * (k + 1) + 1, F - 1] = 127, 255, 127
+    gs[0, 1, 0], us[3, 0, 1], ds[0, 0, 1], ds[2, 1, 0] = -0.01, 0, 0, np.inf
+    s[2, 1], hs[4 * (k + 1), 0] = 0, np.inf
+    q[5], q[5, 200] = 1, 126
+    hq[6 * (k + 1)], hq[6 * (k + 1), 3] = 1, 254
+    with pkg.Context(dims, n_layer=1, max_tokens=1, device=0) as c:
+        dev = _dev(c, g, gs, u, us, q, s, offsets, pairs, np.full((T, k + 1, F), 9.5, np.float32))
+        c.moe_gateup_grouped_fp8(*dev, T)
+        c.sync()
+        h = dev[-1].download(np.float32, (T, k + 1, F))
+        _free(*dev)
+        dev = _dev(c, d, ds, hq, hs, sel, offsets, pairs, np.full((T, k, D), 9.5, np.float32))
+        c.moe_down_grouped_fp8(*dev, T)
+        c.sync()
+        contrib = dev[-1].download(np.float32, (T, k, D))
+        _free(*dev)
+    assert np.all(h[:, k] == 9.5)
+    for e in range(E):
+        p = pairs[offsets[e]:offsets[e + 1]]
+        t, j = (p >> 4).astype(int), (p & 15).astype(int)
+        (wg, bg, _), (wu, bu, _) = _by_blocks(g[e], gs[e], q[t], s[t]), _by_blocks(u[e], us[e], q[t], s[t])
+        want = _silu(wg) * wu
+        assert np.array_equal(np.isnan(h[t, j]), np.isnan(want)), e
+        there = ~np.isnan(want)
+        assert np.all(np.abs(h[t, j] - want)[there] <= _swiglu_bound(wg, wu, bg, bu)[there]), e
+        r = t * (k + 1) + j
+        wd, bd, sure = _by_blocks(d[e], ds[e], hq[r], hs[r])
+        w = sel["w"][t, j].astype(np.float64)[:, None]
+        _same(contrib[t, j], w * wd, w * bd + 2.0**-23 * np.abs(w * wd), sure)
