@@ -194,3 +194,86 @@ def test_a_spoilt_pair_spoils_itself_alone(pkg, T, E, k, D, F):
         wd, bd, sure = _by_blocks(d[e], ds[e], hq[r], hs[r])
         w = sel["w"][t, j].astype(np.float64)[:, None]
         _same(contrib[t, j], w * wd, w * bd + 2.0**-23 * np.abs(w * wd), sure)
+
+
+def _run_gateup_down(c, T, k, D, F, mats, q, s, hq, hs, d_sel, d_off, d_pairs):
+    (g, gs), (u, us), (d, ds) = mats
+    dev = _dev(c, g, gs, u, us, q, s, d, ds, hq, hs, np.full((T, k + 1, F), 9.5, np.float32), np.full((T, k, D), 9.5, np.float32))
+    c.moe_gateup_grouped_fp8(*dev[:6], d_off, d_pairs, dev[10], T)
+    c.moe_down_grouped_fp8(*dev[6:10], d_sel, d_off, d_pairs, dev[11], T)
+    c.sync()
+    got = dev[10].download(np.float32, (T, k + 1, F)), dev[11].download(np.float32, (T, k, D))
+    _free(*dev)
+    return got
+
+
+def _check_pairs(mats, q, s, hq, hs, sel, h, contrib, k, of_expert):
+    """Every slot against 64 bits; of_expert: {expert's place in mats: (tokens, slots)}; all other slots hold 9.5."""
+    (g, gs), (u, us), (d, ds) = mats
+    held = np.ones(h.shape[:2], bool)
+    for e, (t, j) in of_expert.items():
+        held[t, j] = False
+        (wg, bg), (wu, bu) = (ref.product(m[e], ms[e], q[t], s[t]) for m, ms in ((g, gs), (u, us)))
+        assert np.all(np.abs(h[t, j] - _silu(wg) * wu) <= _swiglu_bound(wg, wu, bg, bu)), e
+        r = t * (k + 1) + j
+        wd, bd = ref.product(d[e], ds[e], hq[r], hs[r])
+        w = sel["w"][t, j].astype(np.float64)[:, None]
+        assert np.all(np.abs(contrib[t, j] - w * wd) <= w * bd + 2.0**-23 * np.abs(w * wd)), e
+    assert np.all(h[held] == 9.5) and np.all(contrib[held[:, :k]] == 9.5)
+
+
+def _case(rng, T, E, k, D, F):
+    mats = [ref.weights(rng, *shape, mats=E) for shape in ((F, D), (F, D), (D, F))]
+    return mats, *ref.quantize(rng.standard_normal((T, D)).astype(np.float32)), *ref.quantize(rng.standard_normal((T * (k + 1), F)).astype(np.float32))
+
+
+@pytest.mark.parametrize("T,F", [(7, 256), (130, 256), (130, 768)])
+def test_gateup_and_down_of_lists_with_strangers(pkg, T, F):
+    """Pairs that name a token or a slot that there is none of, an expert whose run ends before it begins, an offset past the list: the rest is computed, nothing else written."""
+    E, k, D = 4, 2, 256
+    assert choice.pairs_as_lanes(False, T, k, E) == choice.pairs_as_lanes(True, T, k, E) == (T == 130)
+    rng = np.random.default_rng(T + F)
+    dims = pkg.synth.Dims(n_embd=D, n_ff=F, n_expert=E, n_used=k)
+    sel, offsets, pairs = _selection(rng, T, E, k)
+    mats, q, s, hq, hs = _case(rng, T, E, k, D, F)
+    good = np.ones(pairs.size, bool)
+    for i, v in ((0, T << 4), (3, 0xFFFFFFF0), (5, 0 << 4 | k), (offsets[3], 0xFFFFFFFF), (pairs.size - 1, 15)):
+        pairs[i], good[i] = v, False
+    offsets[2] = offsets[1] - 1                                # expert 1's run ends before it begins; expert 2 has its pairs and the last of expert 0
+    offsets[4] += 1000
+    of_expert = {}
+    for e in (0, 2, 3):
+        p = np.arange(offsets[e], min(offsets[e + 1], pairs.size))
+        if e == 0:
+            p = p[:-1]                                         # (that one pair is written by both)
+        p = pairs[p[good[p]]]
+        of_expert[e] = (p >> 4).astype(int), (p & 15).astype(int)
+    both = pairs[offsets[1] - 1]
+    with pkg.Context(dims, n_layer=1, max_tokens=1, device=0) as c:
+        dev = _dev(c, sel, offsets, pairs)
+        h, contrib = _run_gateup_down(c, T, k, D, F, mats, q, s, hq, hs, *dev)
+        _free(*dev)
+    if good[offsets[1] - 1]:
+        t, j = int(both >> 4), int(both & 15)
+        of_expert[2] = tuple(np.delete(a, np.flatnonzero((of_expert[2][0] == t) & (of_expert[2][1] == j))) for a in of_expert[2])
+        assert not np.all(h[t, j] == 9.5)
+        h[t, j], contrib[t, j] = 9.5, 9.5
+    _check_pairs(mats, q, s, hq, hs, sel, h, contrib, k, of_expert)
+
+
+@pytest.mark.parametrize("T,F", [(25, 256), (300, 256), (300, 768)])
+def test_gateup_and_down_of_a_shard(pkg, T, F):
+    """A context that holds experts [2, 6) of 8: lists count from the first of them, pairs of the others are not there."""
+    E, k, D, first, count = 8, 3, 256, 2, 4
+    assert choice.pairs_as_lanes(False, T, k, E) == choice.pairs_as_lanes(True, T, k, E) == (T == 300)
+    rng = np.random.default_rng(T + F)
+    dims = pkg.synth.Dims(n_embd=D, n_ff=F, n_expert=E, n_used=k)
+    sel, _, _ = _selection(rng, T, E, k)
+    mats, q, s, hq, hs = _case(rng, T, count, k, D, F)
+    with pkg.Context(dims, n_layer=1, max_tokens=T, device=0, expert_first=first, expert_count=count) as c:
+        d_sel, = _dev(c, sel)
+        d_off, d_pairs = c.alloc((count + 1) * 4), c.alloc(T * k * 4)
+        c.moe_group_pairs(d_sel, T, d_off, d_pairs)
+        h, contrib = _run_gateup_down(c, T, k, D, F, mats, q, s, hq, hs, d_sel, d_off, d_pairs)
+        _free(d_sel, d_off, d_pairs)
+    _check_pairs(mats, q, s, hq, hs, sel, h, contrib, k, {e: np.nonzero(sel["ids"][:, :k] == first + e) for e in range(count)})
