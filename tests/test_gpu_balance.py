@@ -222,3 +222,20 @@ def test_calls_that_overlapped_leave_nothing_behind(contexts):
     for _ in range(2):
         for T, logits, sel, *_ in parts:
             _check(_run(c, logits, sel, None, 0.01, 1.5), _reference(logits, sel["ids"][:, :k], None, 0.01, 1.5), T, E)
+
+
+def test_exponential_over_its_range(contexts):
+    """The gradient of a row of two logits, 0 and -x, where the first expert has every selection: -p0 p1 g, p0 / p1 = e^-x, for x from 0 to the end of the normal numbers.  In halves of
+    an ulp (2^-24 of the value): the exponential 3, as its comment says; the sum of the two 1 and what of the exponential's 3 is in it; its reciprocal 4 (__fdividef); so 12 for p0 and 9 for
+    p1, with the product that makes either; one each for g, p1 g, their difference from zero's and the last product: 25, and what f32 cannot hold, 2^-126."""
+    E, k, T = 2, 1, 1 << 16
+    rng = np.random.default_rng(3)
+    x = np.concatenate([np.linspace(0, 87.3, T - 4096), rng.uniform(0, 1, 2048) * 2.0 ** rng.integers(-20, 0, 2048), np.arange(1, 2049) / 2048 * 87]).astype(np.float32)
+    logits = np.stack([-x, np.zeros_like(x)], 1)
+    sel = _records(rng, T, E, k)
+    sel["ids"][:, 0] = 1
+    _, _, _, grad = _run(contexts(E, k), logits, sel, None, float(T), None)
+    e = np.exp(-x.astype(np.float64))
+    want = -e / (1 + e) ** 2 * 2.0                             # coef * E / (N^2 k) * counts = T * 2 / T^2 * T
+    off = np.abs(grad[:, 0] - want)
+    assert np.all(off <= 25 * 2.0**-24 * np.abs(want) + 2.0**-125), np.max((off - 2.0**-125) / np.abs(want)) * 2**24
