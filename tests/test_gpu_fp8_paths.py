@@ -277,3 +277,60 @@ def test_gateup_and_down_of_a_shard(pkg, T, F):
         h, contrib = _run_gateup_down(c, T, k, D, F, mats, q, s, hq, hs, d_sel, d_off, d_pairs)
         _free(d_sel, d_off, d_pairs)
     _check_pairs(mats, q, s, hq, hs, sel, h, contrib, k, {e: np.nonzero(sel["ids"][:, :k] == first + e) for e in range(count)})
+
+
+def test_two_contexts_at_a_time_write_everything(pkg):
+    """Two contexts' layers on two streams, other inputs every round, every result and everything between spoilt ahead of each: the bits of the calls one after the other."""
+    import torch
+    E, k, D, F, T = 16, 4, 1024, 512, 600
+    assert choice.pairs_as_lanes(True, T, k, E)
+    rng = np.random.default_rng(6)
+    dims = pkg.synth.Dims(n_embd=D, n_ff=F, n_expert=E, n_used=k)
+    sel, offsets, pairs = _selection(rng, T, E, k, 0.1)
+    mats = [t for shape in ((F, D), (F, D), (D, F)) for t in ref.weights(rng, *shape, mats=E)]
+    g, gs, u, us, d, ds, d_sel, d_off, d_pairs = [torch.from_numpy(np.ascontiguousarray(a).view(np.uint8).reshape(-1)).cuda() for a in (*mats, sel, offsets, pairs)]
+    xs, logits = [torch.randn((T, D), device="cuda") for _ in range(3)], [torch.randn((T, E), device="cuda") for _ in range(3)]
+    empty = {"q": ((T, D), torch.uint8), "s": ((T, D // 128), torch.float32), "h": ((T, k + 1, F), torch.float32), "hq": ((T * (k + 1), F), torch.uint8),
+             "hs": ((T * (k + 1), F // 128), torch.float32), "out": ((T, k, D), torch.float32), "y": ((T, E * F), torch.float32), "y2": ((T, D), torch.float32),
+             "counts": ((E + 1,), torch.int32), "probs": ((E,), torch.float32), "loss": ((1,), torch.float32), "grad": ((T, E), torch.float32)}
+    runs = [{n: torch.empty(shape, dtype=t, device="cuda") for n, (shape, t) in empty.items()} for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ctxs = [pkg.Context(dims, n_layer=1, max_tokens=1, device=0) for _ in range(2)]
+    results = ("q", "s", "h", "hq", "hs", "out", "y", "y2", "counts", "probs", "loss", "grad")
+
+    def step(c, b, i):
+        for t in b.values():
+            t.fill_(float("nan") if t.dtype == torch.float32 else 0x5A)
+        c.fp8_quantize(xs[i], T, D, b["q"], b["s"])
+        c.fp8_gemm(g, gs, b["q"], b["s"], b["y"], E * F, D, T)
+        c.moe_gateup_grouped_fp8(g, gs, u, us, b["q"], b["s"], d_off, d_pairs, b["h"], T)
+        c.moe_shared_gateup_fp8(g, gs, u, us, b["q"], b["s"], b["h"], T)
+        c.fp8_quantize(b["h"], T * (k + 1), F, b["hq"], b["hs"])
+        c.moe_down_grouped_fp8(d, ds, b["hq"], b["hs"], d_sel, d_off, d_pairs, b["out"], T)
+        c.moe_shared_down_fp8(d, ds, b["hq"], b["hs"], d_sel, b["y2"], T)
+        c.moe_balance(logits[i], d_sel, None, T, 1.0, b["counts"], b["probs"], b["loss"])
+        c.moe_balance_grad(logits[i], None, b["counts"], T, 1.0, None, b["grad"])
+        return [b[n].clone() for n in results]
+
+    for c, st in zip(ctxs, streams):
+        c.set_stream(st.cuda_stream)
+    torch.cuda.synchronize()
+    want = []
+    for i in range(3):
+        with torch.cuda.stream(streams[0]):
+            want.append(step(ctxs[0], runs[0], i))
+        torch.cuda.synchronize()
+    for w in want:
+        assert not any(torch.isnan(t).any() for t in w if t.dtype == torch.float32)
+    got = []
+    for r in range(9):
+        for x, (c, b, st) in enumerate(zip(ctxs, runs, streams)):
+            with torch.cuda.stream(st):
+                got.append(((r + x) % 3, step(c, b, (r + x) % 3)))
+    torch.cuda.synchronize()
+    for c in ctxs:
+        c.sync()
+        c.close()
+    for i, outs in got:
+        for name, a, w in zip(results, outs, want[i]):
+            assert torch.equal(a, w), name
