@@ -350,14 +350,14 @@ fp8_wide_kernel(const WideArgs a, const __grid_constant__ CUtensorMap x_map, con
     if (any_timed_out && tid == 0) atomicExch(a.status, (uint32_t)kStatusWaitTimeout);
 }
 
-// ---- products grouped by expert (and dense ones of a middling number of rows) --------------------------------------------------
+// ---- products grouped by expert (and dense ones of at most 32 rows) -------------------------------------------------------------
 // Weight rows are the lanes here (M = 128) and a run of at most 32 pairs the columns, as many as there are: the weights are what has to be read.  A unit is
 // the gate and the up rows of one 128-row tile, or two tiles of one matrix, times a run; blocks take consecutive units, so that the runs of an expert
 // with more than 32 pairs read a tile from the L2.  Weight tiles come by TMA, the rows of the pairs with 16-byte copies, each row's scale of a
 // column block beside them; the eight warps that scale and add take the row scales from shared memory.
 //
-// What bounds it: memory, once it runs (gate/up of 16 tokens 32 us, 5.6 TB/s behind 5 us of start: the list of units, the first tiles; the 151,936 x 2048 head 55 us = 5.7 TB/s).  Up to 44 pairs an
-// expert it beats the kernels below (gate/up of 1024 tokens 113 us against 124, down 73 against 96); 64 columns a unit instead of 32 took 121 and 89.
+// What bounds it: memory, once it runs (gate/up of 16 tokens 32 us, 5.6 TB/s behind 5 us of start: the list of units, the first tiles; the 151,936 x 2048 head 55 us = 5.7 TB/s).  Up to some 37
+// pairs an expert (gate/up; down 58) it beats the kernels below; 64 columns a unit instead of 32 took 121 us for gate/up of 1024 tokens, against 113, and 89 for down, against 73.
 namespace gg {
 constexpr int kThreads = 512;                    // warps: 0 weights, 1 MMAs, 2 tensor memory, 4 - 7 rows, 8 - 15 scale and add
 constexpr int kRegAux = 40, kRegRows = 72, kRegAdd = 200;
@@ -474,7 +474,8 @@ __device__ __forceinline__ float silu_times(float g, float u) { return __fdivide
 template <int MODE>
 __global__ void __launch_bounds__(gg::kThreads, 1)
 fp8_group_kernel(const Fp8Args a, const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1) {
-    constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    constexpr bool kGateUp = MODE == kFp8GateUp, kGrouped = MODE != kFp8Dense;   // (of one matrix only a dense product)
+    static_assert(MODE == kFp8Dense || MODE == kFp8GateUp || MODE == kFp8Down, "the shared expert takes other kernels");
     extern __shared__ uint8_t smem_dyn[];
     __shared__ __align__(8) unsigned long long s_bar[2 * gg::kStages + 2 * gg::kSets + 2 * gg::kScales + gg::kMeta];
     __shared__ uint32_t s_tmem;
@@ -1207,7 +1208,7 @@ cudaError_t wide_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
 
 template <int MODE>
 cudaError_t group_launch(const Launch& L, const Fp8Args& a, uint32_t n_sms) {
-    constexpr bool kGateUp = MODE == kFp8GateUp || MODE == kFp8SharedGateUp, kGrouped = MODE == kFp8GateUp || MODE == kFp8Down;
+    constexpr bool kGateUp = MODE == kFp8GateUp, kGrouped = MODE != kFp8Dense;
     if (const cudaError_t e = allow_dynamic_smem<fp8_group_kernel<MODE>>((int)gg::kSmem)) return e;
     if (const cudaError_t e = check_registers<fp8_group_kernel<MODE>, gg::kRegLaunch>()) return e;
     const uint64_t rows = (uint64_t)(kGrouped ? a.n_experts : 1u) * a.M;
