@@ -277,9 +277,9 @@ QKM_API int qkm_dense_gemm(qkm_ctx *c, uint32_t slot, const float *x, uint32_t n
  * lies one after the other, scales too.  Activation rows are E4M3 [n][K] with one f32 scale for each 128 columns,
  * [n][ceil(K/128)]:
  *   y[n][m] = sum over column blocks b of  x_scale[n][b] * w_scale[m/128][b] * (sum over the block's columns of xq * wq)
- * The products of one block are added by the tensor cores, the blocks in f32.  M is any number, K a multiple of 16 (the last block
- * may be short); E4M3 rows start on 16-byte boundaries.  All pointers are DEVICE pointers, scales any f32.  A NaN code makes the sums that it
- * meets NaN, whatever it is multiplied with, and nothing else.
+ * The products of one block are added by the tensor cores, the blocks in f32; the two scales are multiplied first, in f32.  M is any
+ * number, K a multiple of 16 (the last block may be short); E4M3 rows start on 16-byte boundaries.  All pointers are DEVICE pointers,
+ * scales any f32.  A NaN code makes the sums that it meets NaN, whatever it is multiplied with, and nothing else.
  *
  * qkm_fp8_quantize makes such rows: the scale of 128 columns is the smallest power of two (2^-126 at least, 1 for zeros) that keeps
  * their largest finite magnitude at or below 448, so that x / scale is exact and an element is rounded once, to nearest even.
@@ -288,9 +288,11 @@ QKM_API int qkm_fp8_quantize(qkm_ctx *c, const float *x, uint32_t n, uint32_t K,
 QKM_API int qkm_fp8_gemm(qkm_ctx *c, const void *W, const float *w_scale, const void *xq,
                          const float *x_scale, float *y, uint32_t M, uint32_t K, uint32_t n);
 /* The experts' products, as qkm_moe_gateup_grouped, qkm_moe_down_grouped, qkm_moe_shared_gateup and qkm_moe_shared_down with
- * the context's n_embd, n_ff, n_expert and n_used.  xq: the tokens' rows [n_tokens][n_embd]; hq: rows [n_tokens][n_used + 1][n_ff], e.g.
- * qkm_fp8_quantize of h with n = n_tokens * (n_used + 1).  gate/up writes the slots that the list names (the shared form slot n_used),
- * f32; down multiplies by the record's routing weight (w_shared).  h, contrib and y2 start on 16-byte boundaries; n_tokens < 2^27 (rows of qkm_fp8_gemm: 2^28).  Pairs that name a token or a slot that there is none of are skipped. */
+ * the context's n_embd, n_ff, n_expert and n_used (stacks and lists of a context that holds some of the experts: of these).  xq: the
+ * tokens' rows [n_tokens][n_embd]; hq: rows [n_tokens][n_used + 1][n_ff], e.g. qkm_fp8_quantize of h with n = n_tokens * (n_used + 1).
+ * gate/up writes the slots that the list names (the shared form slot n_used),
+ * f32; down multiplies by the record's routing weight (w_shared).  h, contrib and y2 start on 16-byte boundaries; n_tokens < 2^27 (rows
+ * of qkm_fp8_gemm: 2^28).  Pairs that name a token or a slot that there is none of are skipped. */
 QKM_API int qkm_moe_gateup_grouped_fp8(qkm_ctx *c, const void *gate_exps, const float *gate_scale,
                                        const void *up_exps, const float *up_scale, const void *xq,
                                        const float *x_scale, const uint32_t *offsets,
@@ -309,6 +311,7 @@ QKM_API int qkm_moe_shared_down_fp8(qkm_ctx *c, const void *down_shexp, const fl
 /* ---- the router's load (no counterpart in the reference) --------------------------------------------------------------
  * Balance loss of a batch, and what it is made of:
  *   loss = coef * E / (N * n_used) * sum_e counts[e] * probs[e]          (coef where every expert gets the same)
+ * (1 / n_used of the form that adds up the n_used choices without dividing: a coefficient meant for that one is multiplied by n_used.)
  * N: tokens whose mask byte is not zero (mask NULL: all of them); counts[e]: how many of their selections (sel[t].ids[0..n_used), as
  * qkm_moe_select writes them; ids past the table are not counted) name expert e; probs[e]: the mean over these tokens of
  * softmax(logits[t])[e].  A logit that is not finite counts as -3.4e38, as in the selection.  counts: u32[n_expert + 1], the last one N;
